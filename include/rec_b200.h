@@ -45,6 +45,7 @@ enum {
   REC_DEV_COUNTER_TIMEOUT = 2,
   REC_DEV_BAD_TOKEN = 3,
   REC_DEV_BAD_POSITION = 4,
+  REC_DEV_BAD_PAGE = 5, /* a page id outside the pool, or a length past the page table */
 };
 
 /* Scale/bias storage type of quantized weights. */
@@ -502,5 +503,136 @@ REC_API int rec_quantize_affine(const float* w_dev, int64_t n_groups, int32_t bi
  * epilogue with u = 1.  Replaces the engine's `silu` table
  * (megakernel.py:1110-1112: swiglu over every bf16 gate, up = 1). */
 REC_API int rec_silu_table(void* out_dev, void* stream);
+
+/* ---- batched decode over a paged cache ----------------------------------
+ * Several sessions share one pool of pages per layer.  A page holds page_size
+ * rows of every kv head; session b's slot t is row t % page_size of page
+ * table[b][t / page_size].  Row contents are the formats of RecKVLayer: bf16
+ * or fp16 rows (bits 16), or affine group-64 codes with bf16 scales and
+ * biases (bits 8 or 4; K and V may differ).  No counterpart in the reference,
+ * whose engine decodes one session. */
+enum { REC_T_BF16 = 0, REC_T_FP16 = 1, REC_T_FP32 = 2 };
+
+/* Strides are in bytes.  Row starts are 16-byte aligned: k, v and their
+ * strides are multiples of 16.  A row's elements are contiguous.  Scales and
+ * biases of one tensor share their strides (multiples of head_dim / 32
+ * bytes, the size of a row's scales). */
+typedef struct RecPagedKV {
+  void *k, *v;
+  void *k_scales, *k_biases, *v_scales, *v_biases; /* NULL at 16 bits */
+  int64_t k_stride[3], v_stride[3];                /* page, head, row */
+  int64_t k_scale_stride[3], v_scale_stride[3];
+  int32_t n_pages, page_size, n_kv_heads;
+  int32_t head_dim;       /* a multiple of 8 up to 256; of 64 for codes */
+  int32_t k_bits, v_bits; /* both 16, or each 8 or 4 */
+  int32_t dtype;          /* REC_T_BF16 or REC_T_FP16 of 16-bit rows, q and out; codes: REC_T_BF16 */
+} RecPagedKV;
+
+/* The pages of `batch` sessions: table int32 [batch][width], rows
+ * table_stride entries apart.  Entries that no attended or written slot uses
+ * are not read. */
+typedef struct RecPagedTable {
+  const int32_t* table;
+  int64_t table_stride;
+  int32_t width;
+  int32_t batch; /* 1..4096 */
+} RecPagedTable;
+
+/* Writes new tokens' rows.  k_dev, v_dev [rows][n_kv_heads][head_dim] (16
+ * bit; rows row_stride elements apart, contiguous inside; 16-byte aligned);
+ * row r of session b, cu_dev[b] <= r < cu_dev[b + 1], goes to slot
+ * starts_dev[b] + r - cu_dev[b] (K already RoPE'd).  Codes are formed as by
+ * rec_kv_append.  weights (fp32) and positions (int32), both [n_pages]
+ * [n_kv_heads][page_size] or NULL: the written slots get 0 and their slot
+ * number.  A slot outside the table or a page outside the pool sets
+ * *status_dev and that row is not written. */
+REC_API int rec_paged_append(const RecPagedKV* kv, const RecPagedTable* table, const void* k_dev, const void* v_dev,
+                             int64_t k_row_stride, int64_t v_row_stride, int64_t rows, const int32_t* cu_dev,
+                             const int32_t* starts_dev, float* weights, int32_t* positions, int32_t* status_dev,
+                             void* stream);
+
+/* Attention of one new token per session over its lengths[b] slots.
+ *   s_t = scale * q . k_t, or softcap * tanh(s_t / softcap) for softcap > 0;
+ *   t in [max(0, L - window), L) (window 0: all); softmax over them with the
+ *   head's sink logit in the denominator when sinks are given;
+ *   out = sum p_t v_t; a session with no slot gives zeros and lse -inf.
+ * With weights_out, every slot t < L also gets
+ *   weights_out[t] = decay * weights_in[t] + sum of p_t over the kv head's
+ *   query heads   (weights_in may be weights_out; decay 0 reads nothing).
+ * A page outside the pool sets *status_dev and its slots are left out. */
+typedef struct RecPagedAttn {
+  const void* q;            /* [batch][n_q_heads][head_dim], 16-byte aligned */
+  int64_t q_batch_stride, q_head_stride;     /* elements, multiples of 8 */
+  void* out;
+  int64_t out_batch_stride, out_head_stride;
+  float* lse;               /* [batch][n_q_heads] natural log, or NULL */
+  const int32_t* lengths;   /* [batch] */
+  const void* sinks;        /* bf16 [n_q_heads] or NULL */
+  int32_t n_q_heads;        /* a multiple of n_kv_heads */
+  float scale, softcap;
+  int32_t window;
+  const float* weights_in;  /* [n_pages][n_kv_heads][page_size] */
+  float* weights_out;
+  float decay;
+} RecPagedAttn;
+/* Workspace bytes of rec_paged_attn_decode (weights: non-zero when
+ * weights_out is given); 0 for bad arguments.  The first *zeroed bytes have
+ * to be zero before the first call on a workspace; every call leaves them
+ * zero.  Calls that overlap on the GPU need workspaces of their own. */
+REC_API size_t rec_paged_attn_workspace_bytes(const RecPagedKV* kv, const RecPagedTable* table, int32_t n_q_heads,
+                                              int32_t weights, size_t* zeroed);
+REC_API int rec_paged_attn_decode(const RecPagedKV* kv, const RecPagedTable* table, const RecPagedAttn* attn,
+                                  void* workspace, size_t workspace_bytes, int32_t* status_dev, void* stream);
+
+/* Cuts every session's cache to `budget` slots.  Per session and kv head the
+ * slots rank: protected ones first (position >= keep_from[b], or position <
+ * keep_below), then by weight, heaviest first (a NaN weight ranks last), then
+ * by slot; the first min(budget, L) stay.  The evicted slots below the budget,
+ * in ascending order, take the kept rows at or above it, in ascending order
+ * (K, V, scales, biases, weight, position), so only as many rows move as
+ * there are such slots.  positions_in NULL: a slot's position is its number.
+ * weights_out / positions_out / lengths_out may be the inputs; each slot
+ * below min(budget, L) is written, positions_out may be NULL when
+ * positions_in is.  The pages below the budget must belong to one session. */
+typedef struct RecPagedEvict {
+  const int32_t* lengths;
+  int32_t* lengths_out;
+  int32_t budget;
+  const float* weights_in;
+  float* weights_out;
+  const int32_t* positions_in;
+  int32_t* positions_out;
+  const int32_t* keep_from; /* [batch] or NULL */
+  int32_t keep_below;
+} RecPagedEvict;
+REC_API size_t rec_paged_evict_workspace_bytes(const RecPagedKV* kv, const RecPagedTable* table, int32_t budget);
+REC_API int rec_paged_evict(const RecPagedKV* kv, const RecPagedTable* table, const RecPagedEvict* evict,
+                            void* workspace, size_t workspace_bytes, int32_t* status_dev, void* stream);
+
+/* Per-row rules on logits [batch][vocab] (dtype REC_T_*; fp32 arithmetic,
+ * one rounding at the end).  For id i of row b, in this order:
+ *   i in history[b][0 .. len):            x < 0 ? x * repetition : x / repetition
+ *   c = times i is in history[b][prompt .. len): x - frequency * c
+ *   c > 0:                                x - presence
+ *   i in bias_ids[b] (the last entry):    x + its bias
+ *   allow bit clear:                      -inf
+ * history_len / prompt_len NULL: history_cap / 0.  repetition, frequency,
+ * presence: fp32 [batch] or NULL (1, 0, 0).  Ids outside [0, vocab) are
+ * ignored.  logits_out may be logits.  Per row what masked_sampling.py:101-125
+ * applies with one rule for its single session, with counts and biases. */
+typedef struct RecLogitRules {
+  const int32_t* history; /* [batch][history_cap] */
+  int32_t history_cap;    /* < 262,144 */
+  const int32_t* history_len;
+  const int32_t* prompt_len;
+  const float *repetition, *frequency, *presence;
+  const int32_t* bias_ids; /* [batch][n_bias] */
+  const float* bias_values;
+  int32_t n_bias; /* < 8,191 */
+  const uint32_t* allow;
+  int64_t allow_stride; /* words */
+} RecLogitRules;
+REC_API int rec_process_logits(const void* logits, int64_t stride, void* logits_out, int64_t out_stride, int32_t dtype,
+                               int32_t batch, int32_t vocab, const RecLogitRules* rules, void* stream);
 
 #endif /* REC_B200_H */

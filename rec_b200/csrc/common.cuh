@@ -43,6 +43,7 @@ enum : int {
   kStatusCounterTimeout = 2, // a cross-CTA handoff wait ran out
   kStatusBadToken = 3,       // token id outside the vocabulary
   kStatusBadPosition = 4,    // position outside the KV capacity
+  kStatusBadPage = 5,        // page id outside the pool, or a length past the page table
 };
 
 constexpr uint32_t kSpinLimit = 1u << 22;  // polling bound (seconds at most), then give up

@@ -187,6 +187,89 @@ def token_logprob(logits: torch.Tensor, p: abi.RecSampling, ids: torch.Tensor, h
     return res
 
 
+_LOGIT_TYPES = {torch.bfloat16: abi.REC_T_BF16, torch.float16: abi.REC_T_FP16, torch.float32: abi.REC_T_FP32}
+
+
+def _per_row(name: str, x, batch: int, dtype: torch.dtype, device) -> torch.Tensor | None:
+    """A contiguous [batch] tensor of `dtype` (a number is broadcast); None stays."""
+    if x is None:
+        return None
+    if not isinstance(x, torch.Tensor):
+        return torch.full((batch,), x, dtype=dtype, device=device)
+    if x.device != device or x.dtype != dtype or x.shape != (batch,) or not x.is_contiguous():
+        raise ValueError(f"{name} must be a number or a contiguous {dtype} tensor [{batch}] on the logits' device")
+    return x
+
+
+def process_logits(logits: torch.Tensor, history: torch.Tensor | None = None,
+                   history_len: torch.Tensor | None = None, prompt_len: torch.Tensor | None = None,
+                   repetition=None, frequency=None, presence=None, bias_ids: torch.Tensor | None = None,
+                   bias_values: torch.Tensor | None = None, allow: torch.Tensor | None = None,
+                   out: torch.Tensor | None = None) -> torch.Tensor:
+    """The rules of every row of a batch applied to its logits
+    (rec_process_logits): logits bf16, fp16 or fp32 [B, V], rows contiguous
+    inside; the arithmetic is fp32, rounded once.
+
+    history int32 [B, n] with history_len int32 [B] ids in use (default n):
+    ids in it take `repetition` (x < 0 ? x * r : x / r); the c occurrences
+    from prompt_len (int32 [B], default 0) on take `frequency` * c and, once,
+    `presence`.  Each of the three is a number or fp32 [B].  bias_ids int32
+    [B, m] (ids outside the vocabulary, such as -1, are ignored) with
+    bias_values fp32 [B, m] are added, the last entry of an id counting.
+    allow: 32-bit words [B, W], W >= ceil(V / 32), bit i & 31 of word i >> 5
+    set for each allowed id; the others get -inf.  `out` may be `logits`.
+    sample_logits with the penalties off samples from the result."""
+    kind = _LOGIT_TYPES.get(logits.dtype)
+    if kind is None or not logits.is_cuda or logits.dim() != 2 or logits.stride(1) != 1:
+        raise ValueError("logits must be a bf16, fp16 or fp32 CUDA tensor [B, V] with contiguous rows")
+    B, V = logits.shape
+    dev = logits.device
+    if dev.index != torch.cuda.current_device():
+        raise ValueError("the tensors must live on the current CUDA device")
+    if out is None:
+        out = torch.empty_like(logits, memory_format=torch.contiguous_format)
+    elif out.dtype != logits.dtype or out.shape != logits.shape or out.device != dev or out.stride(1) != 1:
+        raise ValueError("out must match the logits, rows contiguous")
+    r = abi.RecLogitRules()
+    keep = []  # what a broadcast number became, until the launch
+    if history is not None:
+        if history.dtype != torch.int32 or history.dim() != 2 or history.shape[0] != B or history.device != dev \
+                or not history.is_contiguous():
+            raise ValueError("history must be a contiguous int32 tensor [B, n] on the logits' device")
+        r.history_cap = history.shape[1]
+        if r.history_cap:
+            r.history = history.data_ptr()
+        if history_len is not None:
+            r.history_len = _per_row("history_len", history_len, B, torch.int32, dev).data_ptr()
+        if prompt_len is not None:
+            r.prompt_len = _per_row("prompt_len", prompt_len, B, torch.int32, dev).data_ptr()
+        for name, x in (("repetition", repetition), ("frequency", frequency), ("presence", presence)):
+            if x is not None:
+                keep.append(_per_row(name, x, B, torch.float32, dev))
+                setattr(r, name, keep[-1].data_ptr())
+    elif history_len is not None or prompt_len is not None:
+        raise ValueError("history_len and prompt_len need a history")
+    if (bias_ids is None) != (bias_values is None):
+        raise ValueError("bias_ids and bias_values come together")
+    if bias_ids is not None:
+        if bias_ids.dtype != torch.int32 or bias_values.dtype != torch.float32 or bias_ids.dim() != 2 \
+                or bias_ids.shape[0] != B or bias_values.shape != bias_ids.shape or bias_ids.device != dev \
+                or bias_values.device != dev or not bias_ids.is_contiguous() or not bias_values.is_contiguous():
+            raise ValueError("bias_ids int32 and bias_values fp32 must be contiguous [B, m] on the logits' device")
+        r.n_bias = bias_ids.shape[1]
+        if r.n_bias:
+            r.bias_ids, r.bias_values = bias_ids.data_ptr(), bias_values.data_ptr()
+    if allow is not None:
+        if allow.element_size() != 4 or allow.dim() != 2 or allow.shape[0] != B or allow.device != dev \
+                or allow.stride(1) != 1 or allow.shape[1] < (V + 31) // 32:
+            raise ValueError("allow must be 32-bit words [B, >= ceil(V / 32)] on the logits' device, rows contiguous")
+        r.allow, r.allow_stride = allow.data_ptr(), allow.stride(0)
+    if B:
+        check(lib().rec_process_logits(logits.data_ptr(), logits.stride(0), out.data_ptr(), out.stride(0), kind, B, V,
+                                       C.byref(r), torch.cuda.current_stream(dev).cuda_stream), "rec_process_logits")
+    return out
+
+
 def filtered_block(engine, state, token, count, seed, *, temperature, top_p, top_k, presence_penalty, grammar=None,
                    logprobs=None, eos=()):
     """ResidentSampler.block on the reference's filtered path
