@@ -523,7 +523,7 @@ typedef struct RecPagedKV {
   int64_t k_stride[3], v_stride[3];                /* page, head, row */
   int64_t k_scale_stride[3], v_scale_stride[3];
   int32_t n_pages, page_size, n_kv_heads;
-  int32_t head_dim;       /* a multiple of 8 up to 256; of 64 for codes */
+  int32_t head_dim;       /* a multiple of 8 up to 256; codes: 64, 128, 256 */
   int32_t k_bits, v_bits; /* both 16, or each 8 or 4 */
   int32_t dtype;          /* REC_T_BF16 or REC_T_FP16 of 16-bit rows, q and out; codes: REC_T_BF16 */
 } RecPagedKV;
@@ -576,13 +576,15 @@ typedef struct RecPagedAttn {
   float decay;
 } RecPagedAttn;
 /* Workspace bytes of rec_paged_attn_decode (weights: non-zero when
- * weights_out is given); 0 for bad arguments.  The first *zeroed bytes have
- * to be zero before the first call on a workspace; every call leaves them
- * zero.  Calls that overlap on the GPU need workspaces of their own. */
+ * weights_out is given); 0 for bad arguments.  *counter_bytes: the size of its
+ * counters, a buffer of their own that is zero before the first call and that
+ * every call, of any shape, leaves zero.  Calls that overlap on the GPU need
+ * a workspace and counters of their own. */
 REC_API size_t rec_paged_attn_workspace_bytes(const RecPagedKV* kv, const RecPagedTable* table, int32_t n_q_heads,
-                                              int32_t weights, size_t* zeroed);
+                                              int32_t weights, size_t* counter_bytes);
 REC_API int rec_paged_attn_decode(const RecPagedKV* kv, const RecPagedTable* table, const RecPagedAttn* attn,
-                                  void* workspace, size_t workspace_bytes, int32_t* status_dev, void* stream);
+                                  void* workspace, size_t workspace_bytes, uint32_t* counters, size_t counter_bytes,
+                                  int32_t* status_dev, void* stream);
 
 /* Cuts every session's cache to `budget` slots.  Per session and kv head the
  * slots rank: protected ones first (position >= keep_from[b], or position <

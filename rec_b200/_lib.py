@@ -87,7 +87,8 @@ _SIGNATURES = {
     "rec_paged_attn_workspace_bytes": (C.c_size_t, [C.POINTER(abi.RecPagedKV), C.POINTER(abi.RecPagedTable), C.c_int32,
                                                     C.c_int32, C.POINTER(C.c_size_t)]),
     "rec_paged_attn_decode": (C.c_int, [C.POINTER(abi.RecPagedKV), C.POINTER(abi.RecPagedTable),
-                                        C.POINTER(abi.RecPagedAttn), C.c_void_p, C.c_size_t, C.c_void_p, C.c_void_p]),
+                                        C.POINTER(abi.RecPagedAttn), C.c_void_p, C.c_size_t, C.c_void_p, C.c_size_t, C.c_void_p,
+                                        C.c_void_p]),
     "rec_paged_evict_workspace_bytes": (C.c_size_t, [C.POINTER(abi.RecPagedKV), C.POINTER(abi.RecPagedTable),
                                                      C.c_int32]),
     "rec_paged_evict": (C.c_int, [C.POINTER(abi.RecPagedKV), C.POINTER(abi.RecPagedTable),

@@ -27,8 +27,9 @@ int paged_view(const RecPagedKV* kv, const RecPagedTable* table, const char* who
                 kv->v_bits);
   REC_CHECK_ARG(kv->dtype == REC_T_BF16 || (wide && kv->dtype == REC_T_FP16),
                 "%s: rows are bf16 or fp16 (quantized caches: bf16)", who);
-  REC_CHECK_ARG(kv->head_dim >= 8 && kv->head_dim <= 256 && kv->head_dim % (codes ? 64 : 8) == 0,
-                "%s: head_dim %d must be a multiple of %d up to 256", who, kv->head_dim, codes ? 64 : 8);
+  REC_CHECK_ARG(codes ? kv->head_dim == 64 || kv->head_dim == 128 || kv->head_dim == 256
+                      : kv->head_dim >= 8 && kv->head_dim <= 256 && kv->head_dim % 8 == 0,
+                "%s: head_dim %d must be a multiple of 8 up to 256 (codes: 64, 128 or 256)", who, kv->head_dim);
   PagedView& p = *out;
   const int d = kv->head_dim;
   const int64_t n[3] = {kv->n_pages, kv->n_kv_heads, kv->page_size};

@@ -116,8 +116,7 @@ def _status_ptr(device: torch.device) -> int | None:
 
 
 def _workspace(call: str, device: torch.device, stream: int, need: int) -> torch.Tensor:
-    """At least `need` bytes, zero when new; the calls leave zero what they
-    need zero."""
+    """At least `need` bytes, zero when new."""
     if torch.cuda.is_current_stream_capturing():
         return torch.zeros(need, dtype=torch.uint8, device=device)
     key = (call, device.index, stream)
@@ -237,11 +236,13 @@ def paged_attn_decode(cache: PagedKV, q: torch.Tensor, table: torch.Tensor, leng
         a.weights_out = _per_slot("weights_out", weights_out, cache, torch.float32)
     a.decay = decay if weights is not None else 0.0
     tr = C.byref(t)
-    need = lib().rec_paged_attn_workspace_bytes(cache._ref, tr, hq, a.weights_out is not None, None)
+    zero = C.c_size_t()
+    need = lib().rec_paged_attn_workspace_bytes(cache._ref, tr, hq, a.weights_out is not None, C.byref(zero))
     stream = _stream(dev)
     ws = _workspace("attn", dev, stream, max(need, 256))
-    check(lib().rec_paged_attn_decode(cache._ref, tr, C.byref(a), ws.data_ptr(), ws.numel(), _status_ptr(dev),
-                                      stream), "rec_paged_attn_decode")
+    counters = _workspace("attn counters", dev, stream, max(zero.value, 4096))  # every call leaves them zero
+    check(lib().rec_paged_attn_decode(cache._ref, tr, C.byref(a), ws.data_ptr(), ws.numel(), counters.data_ptr(),
+                                      counters.numel(), _status_ptr(dev), stream), "rec_paged_attn_decode")
     return out
 
 

@@ -523,3 +523,20 @@ def test_python_refusals():
                 lambda: paged.paged_append(cache, q[:, :2], q[:, :2], t, n, n)):
         with pytest.raises(ValueError):
             bad()
+
+
+def test_attention_shapes_one_after_another():
+    """Calls of different shapes share the scratch: none finds what another
+    left in it."""
+    rng = np.random.default_rng(20)
+    runs = []
+    for heads, d, lengths in ((1, 128, [30000]), (4, 64, [500] * 300), (2, 256, [9000, 1, 4000]), (8, 64, [3] * 400)):
+        lengths = np.asarray(lengths, dtype=np.int32)
+        table, pages = ref.page_table(lengths, 64, rng)
+        k, v = (torch.randn(pages, heads, 64, d, device="cuda").bfloat16() for _ in range(2))
+        q = torch.randn(len(lengths), 8, d, device="cuda").bfloat16()
+        args = (paged.PagedKV(k, v), q, torch.from_numpy(table).cuda(), torch.from_numpy(lengths).cuda())
+        runs.append((args, paged.paged_attn_decode(*args)))
+    for _ in range(3):
+        for args, first in runs:
+            assert torch.equal(paged.paged_attn_decode(*args), first) and bool(torch.isfinite(first).all())

@@ -41,9 +41,9 @@ def attn(**over):
     return a
 
 
-def run_attn(k=None, t=None, a=None, ws=P, nbytes=1 << 30):
+def run_attn(k=None, t=None, a=None, ws=P, nbytes=1 << 30, counters=P, counter_bytes=1 << 20):
     return _lib.lib().rec_paged_attn_decode(C.byref(k or kv()), C.byref(t or table()), C.byref(a or attn()), ws, nbytes,
-                                            None, None)
+                                            counters, counter_bytes, None, None)
 
 
 def run_evict(k=None, t=None, ws=P, nbytes=1 << 30, **over):
@@ -93,8 +93,10 @@ def test_attention(bad):
 
 
 def test_workspaces():
-    need = _lib.lib().rec_paged_attn_workspace_bytes(C.byref(kv()), C.byref(table()), 8, 1, None)
-    assert need > 0
+    zero = C.c_size_t()
+    need = _lib.lib().rec_paged_attn_workspace_bytes(C.byref(kv()), C.byref(table()), 8, 1, C.byref(zero))
+    assert need > 0 and zero.value == 4 * 3 * 2
+    assert run_attn(counters=None) == run_attn(counter_bytes=20) == run_attn(counters=P + 2) == abi.REC_EINVAL
     assert run_attn(nbytes=need - 1, a=attn(weights_out=P)) == abi.REC_EINVAL
     assert run_attn(ws=P + 128) == abi.REC_EINVAL and run_attn(ws=None) == abi.REC_EINVAL
     assert "workspace" in _lib.last_error()
