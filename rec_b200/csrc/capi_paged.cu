@@ -1,4 +1,4 @@
-// Paged cache: argument checks, append and eviction entry points.
+// Paged cache: argument checks and the append.
 #include <limits.h>
 
 #include "paged.cuh"
@@ -155,160 +155,6 @@ __global__ void k_paged_append(const PagedView p, const AppendArgs a) {
   }
 }
 
-// ---------------------------------------------------------------------------
-// Eviction.  One block per (session, kv head): the budget-th largest rank key
-// by bisection over its 32 bits (one count per bit), then holes and survivors
-// listed in slot order, then the rows moved.
-
-struct EvictArgs {
-  const int* lengths;
-  int* lengths_out;
-  int budget;
-  const float* w_in;
-  float* w_out;
-  const int *p_in;
-  int* p_out;
-  const int* keep_from;
-  int keep_below;
-  int* lists;  // [rows][2][cap]: holes, survivors
-  int cap;
-  int* status;
-};
-
-// Ascending in the rank order: 0 for NaN, ..., 0xFFFFFFFF protected.
-__device__ __forceinline__ uint32_t rank_key(float w, bool keep) {
-  if (keep) return 0xFFFFFFFFu;
-  if (w != w) return 0u;
-  const uint32_t u = __float_as_uint(__fadd_rn(w, 0.0f));  // -0 ranks as +0
-  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);       // +inf: 0xFF800000
-}
-
-constexpr int kEvictThreads = 1024;
-
-__device__ int block_sum(int v, int* red) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  v = __reduce_add_sync(0xffffffffu, v);
-  __syncthreads();
-  if (lane == 0) red[warp] = v;
-  __syncthreads();
-  return __reduce_add_sync(0xffffffffu, red[lane]);
-}
-// Exclusive prefix over the block's threads.
-__device__ int block_prefix(int v, int* red) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int x = v;
-  for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, x, o);
-    if (lane >= o) x += y;
-  }
-  __syncthreads();
-  if (lane == 31) red[warp] = x;
-  __syncthreads();
-  int before = 0;
-  for (int w = 0; w < warp; ++w) before += red[w];
-  return before + x - v;
-}
-
-__global__ void __launch_bounds__(kEvictThreads) k_paged_evict(const PagedView p, const EvictArgs a) {
-  __shared__ int red[32];
-  const int b = blockIdx.y, h = blockIdx.x;
-  const int64_t row = int64_t(b) * p.hkv + h;
-  int L = a.lengths[b];
-  if (L < 0 || L > p.slots) {
-    if (threadIdx.x == 0) report(a.status, kStatusBadPage);
-    L = L < 0 ? 0 : int(p.slots);
-  }
-  const int kept = min(L, a.budget);
-  if (h == 0 && threadIdx.x == 0) a.lengths_out[b] = kept;
-  const int from = a.keep_from ? a.keep_from[b] : INT_MAX;
-  auto key = [&](int t) -> uint32_t {
-    int off;
-    const int page = slot_page(p, b, t, off);
-    if (page < 0) {
-      report(a.status, kStatusBadPage);
-      return 0u;
-    }
-    const int64_t at = slot_index(p, page, h, off);
-    const int pos = a.p_in ? a.p_in[at] : t;
-    return rank_key(a.w_in[at], pos >= from || pos < a.keep_below);
-  };
-  // thread i owns the slots [i * run, (i + 1) * run)
-  const int run = (L + kEvictThreads - 1) / kEvictThreads;
-  const int t0 = min(L, int(threadIdx.x) * run), t1 = min(L, t0 + run);
-  uint32_t T = 0;
-  int ties_kept = INT_MAX;
-  if (L > a.budget) {
-    for (int bit = 31; bit >= 0; --bit) {  // the largest T with at least `budget` keys >= T
-      const uint32_t cand = T | (1u << bit);
-      int n = 0;
-      for (int t = t0; t < t1; ++t) n += key(t) >= cand;
-      if (block_sum(n, red) >= a.budget) T = cand;
-    }
-    int n = 0;
-    for (int t = t0; t < t1; ++t) n += key(t) > T;
-    ties_kept = a.budget - block_sum(n, red);
-  }
-  int ties = 0;
-  for (int t = t0; t < t1; ++t) ties += key(t) == T;
-  int tie = block_prefix(ties, red);
-  const int tie0 = tie;
-  auto keep = [&](int t) {
-    const uint32_t k = key(t);
-    return k > T || (k == T && tie++ < ties_kept);
-  };
-  int holes = 0, highs = 0;
-  for (int t = t0; t < t1; ++t) {
-    const bool k = keep(t);
-    holes += t < a.budget && !k;
-    highs += t >= a.budget && k;
-  }
-  int hole = block_prefix(holes, red), high = block_prefix(highs, red);
-  const int moves = block_sum(holes, red);
-  int* dst_list = a.lists + row * 2 * a.cap;
-  int* src_list = dst_list + a.cap;
-  tie = tie0;
-  for (int t = t0; t < t1; ++t) {
-    const bool k = keep(t);
-    if (t < a.budget && !k) dst_list[hole++] = t;
-    if (t >= a.budget && k) src_list[high++] = t;
-  }
-  if (a.w_out != a.w_in || a.p_out != a.p_in)
-    for (int t = threadIdx.x; t < kept; t += kEvictThreads) {
-      int off;
-      const int page = slot_page(p, b, t, off);
-      if (page < 0) continue;
-      const int64_t at = slot_index(p, page, h, off);
-      if (a.w_out != a.w_in) a.w_out[at] = a.w_in[at];
-      if (a.p_out && a.p_out != a.p_in) a.p_out[at] = a.p_in ? a.p_in[at] : t;
-    }
-  __syncthreads();
-  const int lane = threadIdx.x & 31;
-  for (int m = threadIdx.x >> 5; m < moves; m += kEvictThreads / 32) {
-    int od, os;
-    const int dst = dst_list[m], src = src_list[m];
-    const int pd = slot_page(p, b, dst, od), ps = slot_page(p, b, src, os);
-    if (pd < 0 || ps < 0) continue;
-    for (int i = 0; i < 2; ++i) {
-      const PagedRows& r = i ? p.v : p.k;
-      const int bits = i ? p.v_bits : p.k_bits;
-      const uint4* from_row = reinterpret_cast<const uint4*>(row_ptr(r, ps, h, os));
-      uint4* to_row = reinterpret_cast<uint4*>(row_ptr(r, pd, h, od));
-      if (lane < p.d * bits / 128) to_row[lane] = from_row[lane];
-      if (bits != 16 && lane < p.d / 64) {
-        const PagedScales& sc = i ? p.vs : p.ks;
-        const size_t x = scale_at(sc, pd, h, od) + lane, y = scale_at(sc, ps, h, os) + lane;
-        sc.s[x] = sc.s[y];
-        sc.b[x] = sc.b[y];
-      }
-    }
-    if (lane == 0) {
-      const int64_t x = slot_index(p, pd, h, od), y = slot_index(p, ps, h, os);
-      a.w_out[x] = a.w_in[y];
-      if (a.p_out) a.p_out[x] = a.p_in ? a.p_in[y] : src;
-    }
-  }
-}
-
 }  // namespace
 
 REC_API int rec_paged_append(const RecPagedKV* kv, const RecPagedTable* table, const void* k_dev, const void* v_dev,
@@ -331,45 +177,6 @@ REC_API int rec_paged_append(const RecPagedKV* kv, const RecPagedTable* table, c
   const int64_t warps = rows * p.hkv * 2;
   const int64_t blocks = (warps + 7) / 8, most = int64_t(sm_count()) * 8;
   k_paged_append<<<unsigned(blocks < most ? blocks : most), 256, 0, static_cast<cudaStream_t>(stream)>>>(p, a);
-  REC_CHECK_CUDA(cudaGetLastError());
-  return REC_OK;
-}
-
-REC_API size_t rec_paged_evict_workspace_bytes(const RecPagedKV* kv, const RecPagedTable* table, int32_t budget) {
-  if (!kv || !table || budget < 0 || kv->n_kv_heads < 1 || kv->page_size < 1 || table->batch < 1 || table->width < 1)
-    return 0;
-  const int64_t slots = int64_t(table->width) * kv->page_size;
-  const int64_t cap = slots < budget ? slots : budget;
-  return size_t(table->batch) * kv->n_kv_heads * 2 * size_t(cap + 1) * sizeof(int);
-}
-
-REC_API int rec_paged_evict(const RecPagedKV* kv, const RecPagedTable* table, const RecPagedEvict* evict,
-                            void* workspace, size_t workspace_bytes, int32_t* status_dev, void* stream) {
-  PagedView p;
-  const int rc = paged_view(kv, table, "rec_paged_evict", &p);
-  if (rc) return rc;
-  REC_CHECK_ARG(evict && evict->lengths && evict->lengths_out && evict->weights_in && evict->weights_out,
-                "rec_paged_evict: null lengths or weights");
-  REC_CHECK_ARG(!evict->positions_in || evict->positions_out,
-                "rec_paged_evict: positions_in without positions_out");
-  REC_CHECK_ARG(evict->budget >= 0 && evict->keep_below >= 0, "rec_paged_evict: negative budget or keep_below");
-  const size_t need = rec_paged_evict_workspace_bytes(kv, table, evict->budget);
-  REC_CHECK_ARG(workspace && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0,
-                "rec_paged_evict: workspace must be 256-byte aligned and hold %zu bytes", need);
-  EvictArgs a = {};
-  a.lengths = evict->lengths;
-  a.lengths_out = evict->lengths_out;
-  a.budget = evict->budget;
-  a.w_in = evict->weights_in;
-  a.w_out = evict->weights_out;
-  a.p_in = evict->positions_in;
-  a.p_out = evict->positions_out;
-  a.keep_from = evict->keep_from;
-  a.keep_below = evict->keep_below;
-  a.lists = static_cast<int*>(workspace);
-  a.cap = int((p.slots < a.budget ? p.slots : a.budget) + 1);
-  a.status = status_dev;
-  k_paged_evict<<<dim3(p.hkv, p.batch), kEvictThreads, 0, static_cast<cudaStream_t>(stream)>>>(p, a);
   REC_CHECK_CUDA(cudaGetLastError());
   return REC_OK;
 }

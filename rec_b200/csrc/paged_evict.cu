@@ -1,0 +1,383 @@
+// Eviction from a paged cache by accumulated attention weight.
+//
+// Two kernels.  The first selects: a cluster of 1 to 8 blocks per (session,
+// kv head) holds the slots' rank keys in shared memory, finds the budget-th
+// largest by three radix passes (11, 11 and 10 bits; the blocks' histograms
+// meet in distributed shared memory), and lists the evicted slots below the
+// budget and the kept rows at or above it, each in slot order, as (page, row)
+// pairs.  The second moves row r of one list to place r of the other, one
+// 16-byte piece per thread.  Only holes are filled, so a cut of a few tokens
+// moves a few rows; sources are at or above the budget and places below it,
+// so no move reads what another wrote.
+#include <limits.h>
+
+#include "cluster.cuh"
+#include "paged.cuh"
+
+using namespace rec;
+
+namespace {
+
+constexpr int kThreads = 1024;
+constexpr int kWarps = kThreads / 32;
+constexpr int kBins = 2048;
+constexpr int kKeysInShared = 40960;  // of one block: 160 KB
+constexpr int kMaxCluster = 8;
+
+struct EvictArgs {
+  const int* lengths;
+  int* lengths_out;
+  int budget;
+  const float* w_in;
+  float* w_out;
+  const int* p_in;
+  int* p_out;
+  const int* keep_from;
+  int keep_below;
+  int2 *holes, *highs;  // [rows][cap] (page or -1, row of the page)
+  int* high_slot;       // [rows][cap]
+  int* counts;          // [rows]
+  int cap;
+  uint32_t* keys;       // [rows][slots] when a block's keys exceed its shared memory, or NULL
+  int cluster;
+  int* status;
+};
+
+struct SelectSmem {
+  unsigned hist[3][kBins];  // read by the cluster's other blocks
+  int scan[kWarps], scan2[kWarps];
+  int pub[3];               // ties, holes, survivors of this block
+  int digit, want;
+};
+
+// Ascending in the rank order: 0 for NaN, ..., 0xFFFFFFFF protected.
+__device__ __forceinline__ uint32_t rank_key(float w, bool keep) {
+  if (keep) return 0xFFFFFFFFu;
+  if (w != w) return 0u;
+  const uint32_t u = __float_as_uint(__fadd_rn(w, 0.0f));  // -0 ranks as +0
+  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);       // +inf: 0xFF800000
+}
+
+// One more in bin d for every lane that calls with on; lanes of one bin
+// together (weights share their top digits).
+__device__ __forceinline__ void count_digit(unsigned* hist, unsigned d, bool on) {
+  const unsigned same = __match_any_sync(0xffffffffu, on ? d : 0xffffffffu);
+  if (on && (threadIdx.x & 31) == __ffs(same) - 1) atomicAdd(&hist[d], unsigned(__popc(same)));
+}
+
+// Exclusive prefix of the warps' values; all is the block's sum.
+__device__ __forceinline__ int warps_before(int v, int* scan, int& all) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (lane == 0) scan[warp] = v;
+  __syncthreads();
+  int x = scan[lane];
+  all = __reduce_add_sync(0xffffffffu, x);
+  x = lane < warp ? x : 0;
+  return __reduce_add_sync(0xffffffffu, x);
+}
+
+__global__ void __launch_bounds__(kThreads) k_evict_select(const PagedView p, const EvictArgs a) {
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  SelectSmem& sm = *reinterpret_cast<SelectSmem*>(smem_raw);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int row = blockIdx.x / a.cluster, rank = int(cluster_rank()), b = row / p.hkv, h = row - b * p.hkv;
+  int L = a.lengths[b];
+  if (L < 0 || L > p.slots) {
+    if (threadIdx.x == 0) report(a.status, kStatusBadPage);
+    L = L < 0 ? 0 : int(p.slots);
+  }
+  const int budget = a.budget, kept = min(L, budget);
+  const bool copies = a.w_out != a.w_in || a.p_out != a.p_in;
+  auto copy_slot = [&](int t) {  // slot t stays where it is
+    int off;
+    const int page = slot_page(p, b, t, off);
+    if (page < 0) return;
+    const int64_t at = slot_index(p, page, h, off);
+    if (a.w_out != a.w_in) a.w_out[at] = a.w_in[at];
+    if (a.p_out && a.p_out != a.p_in) a.p_out[at] = a.p_in ? a.p_in[at] : t;
+  };
+  if (L <= budget || budget == 0) {  // the same for the whole cluster
+    if (rank == 0 && threadIdx.x == 0) a.counts[row] = 0;
+    if (copies)
+      for (int t = rank * kThreads + threadIdx.x; t < kept; t += a.cluster * kThreads) copy_slot(t);
+    return;
+  }
+  // this block's slots: [s0, s0 + n)
+  const int slice = ((L + a.cluster - 1) / a.cluster + 31) & ~31;
+  const int s0 = min(L, rank * slice), n = min(L, s0 + slice) - s0;
+  uint32_t* keys = a.keys ? a.keys + int64_t(row) * p.slots + s0
+                          : reinterpret_cast<uint32_t*>(smem_raw + sizeof(SelectSmem));
+  for (int i = threadIdx.x; i < 3 * kBins; i += kThreads) (&sm.hist[0][0])[i] = 0u;
+  __syncthreads();
+  const int from = a.keep_from ? a.keep_from[b] : INT_MAX;
+  for (int i0 = 0; i0 < n; i0 += kThreads) {
+    const int i = i0 + threadIdx.x;
+    uint32_t key = 0u;
+    if (i < n) {
+      int off;
+      const int t = s0 + i, page = slot_page(p, b, t, off);
+      if (page < 0) {
+        report(a.status, kStatusBadPage);
+      } else {
+        const int64_t at = slot_index(p, page, h, off);
+        const int pos = a.p_in ? a.p_in[at] : t;
+        key = rank_key(a.w_in[at], pos >= from || pos < a.keep_below);
+      }
+      keys[i] = key;
+    }
+    count_digit(sm.hist[0], key >> 21, i < n);
+  }
+  // the budget-th largest key T, and how many of its equals stay
+  uint32_t T = 0;
+  int want = budget;
+#pragma unroll 1
+  for (int pass = 0; pass < 3; ++pass) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+    const unsigned bins = pass == 2 ? 1024u : 2048u;
+    if (pass > 0)
+      for (int i0 = 0; i0 < n; i0 += kThreads) {
+        const int i = i0 + threadIdx.x;
+        const uint32_t key = i < n ? keys[i] : 0u;
+        const int above = pass == 1 ? 21 : 10;
+        count_digit(sm.hist[pass], (key >> shift) & (bins - 1), i < n && (key >> above) == (T >> above));
+      }
+    cluster_sync_all();
+    // thread i sums bins 2(1023 - i) + 1 and 2(1023 - i): descending order
+    const int d = 2 * (kThreads - 1 - int(threadIdx.x));
+    int c1 = 0, c0 = 0;
+    for (int r = 0; r < a.cluster; ++r) {
+      const uint2 c = *reinterpret_cast<const uint2*>(peer(&sm.hist[pass][d], r));
+      c0 += int(c.x);
+      c1 += int(c.y);
+    }
+    int x = c0 + c1;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    int all;
+    const int before = warps_before(__shfl_sync(0xffffffffu, x, 31), sm.scan, all) + x - c0 - c1;
+    if (before < want && want <= before + c0 + c1) {
+      const bool upper = want <= before + c1;
+      sm.digit = upper ? d + 1 : d;
+      sm.want = want - before - (upper ? 0 : c1);
+    }
+    __syncthreads();
+    T |= uint32_t(sm.digit) << shift;
+    want = sm.want;
+    __syncthreads();
+  }
+  // a warp's slots are contiguous, so ranks in slot order are prefix counts
+  const int chunk = ((n + kWarps - 1) / kWarps + 31) & ~31;
+  const int i_lo = min(n, warp * chunk), i_hi = min(n, i_lo + chunk);
+  int ties = 0;
+  for (int i0 = i_lo; i0 < i_hi; i0 += 32)
+    ties += __popc(__ballot_sync(0xffffffffu, i0 + lane < i_hi && keys[i0 + lane] == T));
+  int all;
+  int tie0 = warps_before(ties, sm.scan, all);
+  if (threadIdx.x == 0) sm.pub[0] = all;
+  cluster_sync_all();
+  for (int r = 0; r < rank; ++r) tie0 += *peer(&sm.pub[0], r);
+  const unsigned below = (1u << lane) - 1u;
+  // keep / hole / survivor of the 32 slots from i0; tie counts on
+  auto classify = [&](int i0, int& tie, bool& keep, bool& hole, bool& high) {
+    const int i = i0 + lane, t = s0 + i;
+    const bool in = i < i_hi;
+    const uint32_t key = in ? keys[i] : 0u;
+    const unsigned eq = __ballot_sync(0xffffffffu, in && key == T);
+    keep = in && (key > T || (key == T && tie + __popc(eq & below) < want));
+    tie += __popc(eq);
+    hole = in && !keep && t < budget;
+    high = keep && t >= budget;
+  };
+  int holes = 0, highs = 0, tie = tie0;
+  for (int i0 = i_lo; i0 < i_hi; i0 += 32) {
+    bool keep, hole, high;
+    classify(i0, tie, keep, hole, high);
+    holes += __popc(__ballot_sync(0xffffffffu, hole));
+    highs += __popc(__ballot_sync(0xffffffffu, high));
+  }
+  int hole_at = warps_before(holes, sm.scan, all);
+  if (threadIdx.x == 0) sm.pub[1] = all;
+  int high_at = warps_before(highs, sm.scan2, all);
+  if (threadIdx.x == 0) sm.pub[2] = all;
+  cluster_sync_all();
+  int moves = 0;
+  for (int r = 0; r < a.cluster; ++r) {
+    const int x = *peer(&sm.pub[1], r), y = *peer(&sm.pub[2], r);
+    moves += x;
+    if (r < rank) {
+      hole_at += x;
+      high_at += y;
+    }
+  }
+  if (rank == 0 && threadIdx.x == 0) a.counts[row] = moves;
+  int2* hole_list = a.holes + int64_t(row) * a.cap;
+  int2* high_list = a.highs + int64_t(row) * a.cap;
+  int* slot_list = a.high_slot + int64_t(row) * a.cap;
+  tie = tie0;
+  for (int i0 = i_lo; i0 < i_hi; i0 += 32) {
+    bool keep, hole, high;
+    classify(i0, tie, keep, hole, high);
+    const unsigned ho = __ballot_sync(0xffffffffu, hole), hi = __ballot_sync(0xffffffffu, high);
+    const int t = s0 + i0 + lane;
+    if (hole || high) {
+      int off;
+      const int page = slot_page(p, b, t, off);
+      const int at = hole ? hole_at + __popc(ho & below) : high_at + __popc(hi & below);
+      (hole ? hole_list : high_list)[at] = make_int2(page, off);
+      if (high) slot_list[at] = t;
+    } else if (keep && copies) {
+      copy_slot(t);
+    }
+    hole_at += __popc(ho);
+    high_at += __popc(hi);
+  }
+  cluster_sync_all();  // a block's counts stay readable until every block has them
+}
+
+constexpr int kMoveThreads = 256;
+
+// Piece i of move m: the 16-byte pieces of K, of V, the scales and biases of
+// K and V (codes), then the weight and position.
+__global__ void __launch_bounds__(kMoveThreads) k_evict_move(const PagedView p, const EvictArgs a, const FastDiv per) {
+  grid_wait();  // launched while the selection ends
+  const int row = blockIdx.y, b = row / p.hkv, h = row - b * p.hkv;
+  if (blockIdx.x == 0 && h == 0 && threadIdx.x == 0) {
+    const int64_t L = max(0, a.lengths[b]);
+    a.lengths_out[b] = int(min(min(L, p.slots), int64_t(a.budget)));
+  }
+  const int moves = a.counts[row];
+  const int2* hole_list = a.holes + int64_t(row) * a.cap;
+  const int2* high_list = a.highs + int64_t(row) * a.cap;
+  const int nk = p.d * p.k_bits / 128, nv = p.d * p.v_bits / 128;
+  const int groups = p.k_bits == 16 ? 0 : p.d / 64;
+  const int64_t pieces = int64_t(moves) * per.d;
+  const int step = gridDim.x * kMoveThreads;
+  for (int64_t x = int64_t(blockIdx.x) * kMoveThreads + threadIdx.x; x < pieces; x += step) {
+    const int m = x < INT_MAX ? int(fdiv(uint32_t(x), per)) : int(x / per.d);
+    int i = int(x - int64_t(m) * per.d);
+    const int2 to = hole_list[m], from = high_list[m];
+    if (to.x < 0 || from.x < 0) continue;
+    if (i < nk + nv) {
+      const PagedRows& r = i < nk ? p.k : p.v;
+      if (i >= nk) i -= nk;
+      reinterpret_cast<uint4*>(row_ptr(r, to.x, h, to.y))[i] =
+          reinterpret_cast<const uint4*>(row_ptr(r, from.x, h, from.y))[i];
+    } else if (i < int(per.d) - 1) {
+      i -= nk + nv;
+      const PagedScales& s = i < 2 ? p.ks : p.vs;
+      uint16_t* base = i & 1 ? s.b : s.s;
+      uint16_t* dst = base + scale_at(s, to.x, h, to.y);
+      const uint16_t* src = base + scale_at(s, from.x, h, from.y);
+      if (groups == 1) *dst = *src;
+      else if (groups == 2) *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(src);
+      else *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(src);
+    } else {
+      const int64_t dst = slot_index(p, to.x, h, to.y), src = slot_index(p, from.x, h, from.y);
+      a.w_out[dst] = a.w_in[src];
+      if (a.p_out) a.p_out[dst] = a.p_in ? a.p_in[src] : a.high_slot[int64_t(row) * a.cap + m];
+    }
+  }
+}
+
+struct EvictLayout {
+  int cluster, cap;
+  bool shared;  // the keys fit shared memory
+  size_t holes, highs, slots, counts, keys, total;
+};
+EvictLayout evict_layout(int64_t slots, int batch, int hkv, int budget) {
+  EvictLayout l;
+  const int64_t rows = int64_t(batch) * hkv;
+  auto slice = [&](int c) { return ((slots + c - 1) / c + 31) / 32 * 32; };
+  // more blocks per row while the rows leave SMs idle and a block has more than 1,024 keys
+  l.cluster = 1;
+  while (l.cluster < kMaxCluster && (slice(l.cluster) > kKeysInShared ||
+                                     (rows * l.cluster < 148 && slice(l.cluster) > 1024)))
+    l.cluster *= 2;
+  l.shared = slice(l.cluster) <= kKeysInShared;
+  l.cap = int(slots < budget ? slots : budget);
+  auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+  l.holes = 0;
+  l.highs = up(size_t(rows) * l.cap * 8);
+  l.slots = 2 * l.highs;
+  l.counts = l.slots + up(size_t(rows) * l.cap * 4);
+  l.keys = l.counts + up(size_t(rows) * 4);
+  l.total = l.keys + (l.shared ? 0 : up(size_t(rows) * size_t(slots) * 4));
+  return l;
+}
+
+}  // namespace
+
+REC_API size_t rec_paged_evict_workspace_bytes(const RecPagedKV* kv, const RecPagedTable* table, int32_t budget) {
+  if (!kv || !table || budget < 0 || kv->n_kv_heads < 1 || kv->page_size < 1 || table->batch < 1 || table->width < 1)
+    return 0;
+  return evict_layout(int64_t(table->width) * kv->page_size, table->batch, kv->n_kv_heads, budget).total;
+}
+
+REC_API int rec_paged_evict(const RecPagedKV* kv, const RecPagedTable* table, const RecPagedEvict* evict,
+                            void* workspace, size_t workspace_bytes, int32_t* status_dev, void* stream) {
+  PagedView p;
+  const int rc = paged_view(kv, table, "rec_paged_evict", &p);
+  if (rc) return rc;
+  REC_CHECK_ARG(evict && evict->lengths && evict->lengths_out && evict->weights_in && evict->weights_out,
+                "rec_paged_evict: null lengths or weights");
+  REC_CHECK_ARG(!evict->positions_in || evict->positions_out,
+                "rec_paged_evict: positions_in without positions_out");
+  REC_CHECK_ARG(evict->budget >= 0 && evict->keep_below >= 0, "rec_paged_evict: negative budget or keep_below");
+  const EvictLayout l = evict_layout(p.slots, p.batch, p.hkv, evict->budget);
+  REC_CHECK_ARG(workspace && workspace_bytes >= l.total && (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0,
+                "rec_paged_evict: workspace must be 256-byte aligned and hold %zu bytes", l.total);
+  const int rows = p.batch * p.hkv;  // <= 4096 * 1024
+  REC_CHECK_ARG(rows <= 65535, "rec_paged_evict: %d sessions times kv heads (at most 65,535)", rows);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  EvictArgs a = {};
+  a.lengths = evict->lengths;
+  a.lengths_out = evict->lengths_out;
+  a.budget = evict->budget;
+  a.w_in = evict->weights_in;
+  a.w_out = evict->weights_out;
+  a.p_in = evict->positions_in;
+  a.p_out = evict->positions_out;
+  a.keep_from = evict->keep_from;
+  a.keep_below = evict->keep_below;
+  a.holes = reinterpret_cast<int2*>(ws + l.holes);
+  a.highs = reinterpret_cast<int2*>(ws + l.highs);
+  a.high_slot = reinterpret_cast<int*>(ws + l.slots);
+  a.counts = reinterpret_cast<int*>(ws + l.counts);
+  a.cap = l.cap;
+  a.keys = l.shared ? nullptr : reinterpret_cast<uint32_t*>(ws + l.keys);
+  a.cluster = l.cluster;
+  a.status = status_dev;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const size_t slice = size_t((p.slots + l.cluster - 1) / l.cluster + 31) / 32 * 32;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(rows * l.cluster);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = sizeof(SelectSmem) + (l.shared ? slice * 4 : 0);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim = {unsigned(l.cluster), 1, 1};
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  REC_CHECK_CUDA(set_smem_limit(reinterpret_cast<const void*>(&k_evict_select),
+                                sizeof(SelectSmem) + size_t(kKeysInShared) * 4));
+  REC_CHECK_CUDA(cudaLaunchKernelEx(&cfg, k_evict_select, p, a));
+  const unsigned per = unsigned(p.d * (p.k_bits + p.v_bits) / 128 + (p.k_bits == 16 ? 0 : 4) + 1);
+  // blocks per row: two waves of the SMs over all rows, no more than a full list needs
+  const int64_t most = (int64_t(l.cap) * per + kMoveThreads - 1) / kMoveThreads;
+  int64_t x = (int64_t(sm_count()) * 16 + rows - 1) / rows;
+  x = x < most ? x : most;
+  cudaLaunchConfig_t mv = {};
+  mv.gridDim = dim3(unsigned(x < 1 ? 1 : x), rows);
+  mv.blockDim = dim3(kMoveThreads);
+  mv.stream = st;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  mv.attrs = attr;
+  mv.numAttrs = 1;
+  REC_CHECK_CUDA(cudaLaunchKernelEx(&mv, k_evict_move, p, a, make_fastdiv(per)));
+  return REC_OK;
+}
