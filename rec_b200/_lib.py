@@ -81,20 +81,18 @@ _SIGNATURES = {
     "rec_schedule_for": (C.c_int32, [C.c_void_p, C.c_int32]),
     "rec_set_profile": (C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t]),
     "rec_set_layer_profile": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int32]),
-    "rec_paged_append": (C.c_int, [C.POINTER(abi.RecPagedKV), C.POINTER(abi.RecPagedTable), C.c_void_p, C.c_void_p,
-                                   C.c_int64, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
-                                   C.c_void_p, C.c_void_p]),
-    "rec_paged_attn_workspace_bytes": (C.c_size_t, [C.POINTER(abi.RecPagedKV), C.POINTER(abi.RecPagedTable), C.c_int32,
-                                                    C.c_int32, C.POINTER(C.c_size_t)]),
-    "rec_paged_attn_decode": (C.c_int, [C.POINTER(abi.RecPagedKV), C.POINTER(abi.RecPagedTable),
-                                        C.POINTER(abi.RecPagedAttn), C.c_void_p, C.c_size_t, C.c_void_p, C.c_size_t, C.c_void_p,
-                                        C.c_void_p]),
-    "rec_paged_evict_workspace_bytes": (C.c_size_t, [C.POINTER(abi.RecPagedKV), C.POINTER(abi.RecPagedTable),
-                                                     C.c_int32]),
-    "rec_paged_evict": (C.c_int, [C.POINTER(abi.RecPagedKV), C.POINTER(abi.RecPagedTable),
-                                  C.POINTER(abi.RecPagedEvict), C.c_void_p, C.c_size_t, C.c_void_p, C.c_void_p]),
+    # structures of the batched calls: a ctypes reference or their packed bytes
+    "rec_paged_append": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.c_int64,
+                                   C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "rec_paged_attn_workspace_bytes": (C.c_size_t, [C.c_void_p, C.c_void_p, C.c_int32, C.c_int32,
+                                                    C.POINTER(C.c_size_t)]),
+    "rec_paged_attn_decode": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p,
+                                        C.c_size_t, C.c_void_p, C.c_void_p]),
+    "rec_paged_evict_workspace_bytes": (C.c_size_t, [C.c_void_p, C.c_void_p, C.c_int32]),
+    "rec_paged_evict": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p,
+                                  C.c_void_p]),
     "rec_process_logits": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_int32, C.c_int32, C.c_int32,
-                                     C.POINTER(abi.RecLogitRules), C.c_void_p]),
+                                     C.c_void_p, C.c_void_p]),
 }
 
 

@@ -13,6 +13,13 @@ from . import abi
 from ._lib import check, lib
 
 
+# The current device and the raw handle of its current stream, without the
+# objects that torch.cuda's public calls build (a microsecond or two per call).
+current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _stream() -> C.c_void_p:
     return C.c_void_p(torch.cuda.current_stream().cuda_stream)
 

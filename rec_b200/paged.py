@@ -15,15 +15,32 @@ its scratch from the capture's own pool.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 import torch
 
 from . import abi
 from ._lib import check, lib
+from .ops import current_device as _current_device, raw_stream as _raw_stream
 
 _TYPES = {torch.bfloat16: abi.REC_T_BF16, torch.float16: abi.REC_T_FP16}
-_status: dict[int, torch.Tensor] = {}  # one word per device
-_scratch: dict[tuple, torch.Tensor] = {}  # (call, device, stream)
+_status: dict[int, tuple] = {}  # device -> (one word, its address)
+_scratch: dict[tuple, tuple] = {}  # (call, device, stream) -> (tensors, addresses and sizes)
+_sizes: dict[tuple, tuple] = {}  # shape of a call -> scratch bytes
+
+# The C structures of abi.py as one pack each: a step makes these calls once
+# per layer, and filling a ctypes structure field by field costs several
+# microseconds of it.
+_KV = struct.Struct("@6P12q7i4x")
+_TABLE = struct.Struct("@Pq2i")
+_ATTN = struct.Struct("@Pqq Pqq 3P i2fi 2P f4x".replace(" ", ""))
+_EVICT = struct.Struct("@2Pi4x5Pi4x")
+for _pack, _type in ((_KV, abi.RecPagedKV), (_TABLE, abi.RecPagedTable), (_ATTN, abi.RecPagedAttn),
+                     (_EVICT, abi.RecPagedEvict)):
+    assert _pack.size == C.sizeof(_type), _type
+
+_bf16, _f32, _i32 = torch.bfloat16, torch.float32, torch.int32
+_capturing = torch.cuda.is_current_stream_capturing
 
 
 class PagedKV:
@@ -36,53 +53,45 @@ class PagedKV:
     Only the last dimension has to be contiguous; row starts are 16-byte
     aligned.  A view: the tensors stay the caller's."""
 
-    __slots__ = ("k", "v", "scales", "device", "dtype", "shape", "head_dim", "desc", "_ref")
+    __slots__ = ("k", "v", "scales", "device", "dtype", "shape", "head_dim", "bits", "_desc", "_index")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scales: torch.Tensor | None = None,
                  k_biases: torch.Tensor | None = None, v_scales: torch.Tensor | None = None,
                  v_biases: torch.Tensor | None = None):
-        scales = (k_scales, k_biases, v_scales, v_biases)
-        kd, vd = k.shape, v.shape
-        if len(kd) != 4 or len(vd) != 4 or kd[:3] != vd[:3] or not k.is_cuda or k.device != v.device:
+        kd, vd, dtype, dev = k.shape, v.shape, k.dtype, k.device
+        if len(kd) != 4 or len(vd) != 4 or kd[:3] != vd[:3] or dev.type != "cuda" or v.device != dev:
             raise ValueError("k and v must be CUDA tensors [pages, kv heads, page_size, ...] of the same pages")
-        d = abi.RecPagedKV()
-        ks, vs = k.stride(), v.stride()
-        if ks[3] != 1 or vs[3] != 1:
+        (k0, k1, k2, k3), (v0, v1, v2, v3) = k.stride(), v.stride()
+        if k3 != 1 or v3 != 1:
             raise ValueError("the rows of k and v must be contiguous")
-        if k.dtype in _TYPES:
-            if v.dtype != k.dtype or kd != vd or any(t is not None for t in scales):
+        self.scales = scales = (k_scales, k_biases, v_scales, v_biases)
+        kind = _TYPES.get(dtype)
+        if kind is not None:
+            if v.dtype != dtype or kd != vd or scales != (None, None, None, None):
                 raise ValueError("16-bit pools: k and v of one type and shape, no scales")
-            self.head_dim, self.dtype, item = kd[3], k.dtype, 2
-            d.k_bits = d.v_bits = 16
-            d.dtype = _TYPES[k.dtype]
+            self.head_dim, self.dtype, self.bits = kd[3], dtype, (16, 16)
+            self._desc = _KV.pack(k.data_ptr(), v.data_ptr(), 0, 0, 0, 0, 2 * k0, 2 * k1, 2 * k2, 2 * v0, 2 * v1, 2 * v2,
+                                  0, 0, 0, 0, 0, 0, kd[0], kd[2], kd[1], kd[3], 16, 16, kind)
         else:
             if k.element_size() != 4 or v.element_size() != 4 or any(t is None for t in scales):
                 raise ValueError("pools must be bf16, fp16, or 32-bit code words with scales and biases")
             groups = k_scales.shape[-1]
-            self.head_dim, self.dtype, item = 64 * groups, torch.bfloat16, 4
-            for t, like in zip(scales, (k_scales, k_scales, v_scales, v_scales)):
-                if t.dtype != torch.bfloat16 or t.shape != (*kd[:3], groups) or t.device != k.device \
-                        or t.stride() != like.stride() or t.stride(3) != 1:
+            want = (*kd[:3], groups)
+            a, b = k_scales.stride(), v_scales.stride()
+            for t, st in ((k_scales, a), (k_biases, a), (v_scales, b), (v_biases, b)):
+                if t.dtype != _bf16 or t.shape != want or t.device != dev or t.stride() != st or st[3] != 1:
                     raise ValueError("scales and biases must be bf16 [pages, kv heads, page_size, head_dim / 64], "
                                      "those of one tensor with the same strides")
             if groups < 1 or kd[3] % (2 * groups) or vd[3] % (2 * groups):
                 raise ValueError("code words do not match the scales' head_dim")
-            d.k_bits, d.v_bits = kd[3] // (2 * groups), vd[3] // (2 * groups)
-            d.dtype = abi.REC_T_BF16
-            a, b = k_scales.stride(), v_scales.stride()
-            d.k_scale_stride[:] = (2 * a[0], 2 * a[1], 2 * a[2])
-            d.v_scale_stride[:] = (2 * b[0], 2 * b[1], 2 * b[2])
-            d.k_scales, d.k_biases = k_scales.data_ptr(), k_biases.data_ptr()
-            d.v_scales, d.v_biases = v_scales.data_ptr(), v_biases.data_ptr()
-        d.k, d.v = k.data_ptr(), v.data_ptr()
-        d.k_stride[:] = (item * ks[0], item * ks[1], item * ks[2])
-        d.v_stride[:] = (item * vs[0], item * vs[1], item * vs[2])
-        d.n_pages, d.n_kv_heads, d.page_size = kd[0], kd[1], kd[2]
-        d.head_dim = self.head_dim
-        self.k, self.v, self.scales, self.device = k, v, scales, k.device
-        self.shape = tuple(kd[:3])
-        self.desc = d
-        self._ref = C.byref(d)
+            self.head_dim, self.dtype = 64 * groups, _bf16
+            self.bits = kb, vb = kd[3] // (2 * groups), vd[3] // (2 * groups)
+            self._desc = _KV.pack(
+                k.data_ptr(), v.data_ptr(), k_scales.data_ptr(), k_biases.data_ptr(), v_scales.data_ptr(),
+                v_biases.data_ptr(), 4 * k0, 4 * k1, 4 * k2, 4 * v0, 4 * v1, 4 * v2, 2 * a[0], 2 * a[1], 2 * a[2],
+                2 * b[0], 2 * b[1], 2 * b[2], kd[0], kd[2], kd[1], 64 * groups, kb, vb, abi.REC_T_BF16)
+        self.k, self.v, self.device, self._index = k, v, dev, dev.index
+        self.shape = kd[:3]
 
     @classmethod
     def allocate(cls, pages: int, kv_heads: int, page_size: int, head_dim: int, *, k_bits: int = 16, v_bits: int = 16,
@@ -99,31 +108,38 @@ class PagedKV:
                              for _ in range(4)))
 
 
-def _stream(device: torch.device) -> int:
-    if device.index != torch.cuda.current_device():
+def _stream(index: int) -> int:
+    if index != _current_device():
         raise ValueError("the tensors must live on the current CUDA device")
-    return torch.cuda.current_stream(device).cuda_stream
+    return _raw_stream(index)
 
 
-def _status_ptr(device: torch.device) -> int | None:
-    t = _status.get(device.index)
-    if t is None:
-        if torch.cuda.is_current_stream_capturing():
+def _status_ptr(index: int) -> int | None:
+    s = _status.get(index)
+    if s is None:
+        if _capturing():
             return None  # cleared by every replay if it were captured
-        t = _status[device.index] = torch.zeros(1, dtype=torch.int32, device=device)
-        torch.cuda.current_stream(device).synchronize()  # zero before any other stream's call
-    return t.data_ptr()
+        t = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", index))
+        torch.cuda.current_stream(index).synchronize()  # zero before any other stream's call
+        s = _status[index] = (t, t.data_ptr())
+    return s[1]
 
 
-def _workspace(call: str, device: torch.device, stream: int, need: int) -> torch.Tensor:
-    """At least `need` bytes, zero when new."""
-    if torch.cuda.is_current_stream_capturing():
-        return torch.zeros(need, dtype=torch.uint8, device=device)
-    key = (call, device.index, stream)
-    t = _scratch.get(key)
-    if t is None or t.numel() < need:
-        t = _scratch[key] = torch.zeros(need, dtype=torch.uint8, device=device)
-    return t
+def _buffers(call: str, device: torch.device, index: int, stream: int, need: int, zero: int) -> tuple:
+    """(address, bytes, address, bytes) of the call's workspace and of its
+    counters, which are zero between calls."""
+    s = _scratch.get((call, index, stream))
+    if s is not None and s[1][1] >= need and s[1][3] >= zero and not _capturing():
+        return s[1]
+    need, zero = max(need, 256), max(zero, 4096)
+    if s is not None:
+        need, zero = max(need, s[1][1]), max(zero, s[1][3])
+    ws = torch.empty(need, dtype=torch.uint8, device=device)
+    counters = torch.zeros(zero, dtype=torch.uint8, device=device)
+    at = (ws.data_ptr(), need, counters.data_ptr(), zero)
+    if not _capturing():
+        _scratch[(call, index, stream)] = ((ws, counters), at)
+    return at
 
 
 def check_status(device=None) -> None:
@@ -131,30 +147,32 @@ def check_status(device=None) -> None:
     check met a bad page id or slot; clears the record."""
     index = torch.device("cuda" if device is None else device).index
     index = torch.cuda.current_device() if index is None else index
-    t = _status.get(index)
-    if t is None:
+    s = _status.get(index)
+    if s is None:
         return
     torch.cuda.synchronize(index)
-    code = int(t.item())
+    code = int(s[0].item())
     if code:
-        t.zero_()
+        s[0].zero_()
         check(code)
 
 
-def _table(table: torch.Tensor, device: torch.device) -> abi.RecPagedTable:
-    if table.dtype != torch.int32 or table.dim() != 2 or table.device != device or table.stride(1) != 1:
+def _table(table: torch.Tensor, device: torch.device) -> tuple:
+    """(the packed table, batch, width)."""
+    if table.dtype != _i32 or table.device != device or table.dim() != 2 or table.stride(1) != 1:
         raise ValueError("the page table must be int32 [batch, pages] on the cache's device, rows contiguous")
-    return abi.RecPagedTable(table.data_ptr(), table.stride(0), table.shape[1], table.shape[0])
+    batch, width = table.shape
+    return _TABLE.pack(table.data_ptr(), table.stride(0), width, batch), batch, width
 
 
 def _ints(name: str, t: torch.Tensor, n: int, device: torch.device) -> int:
-    if t.dtype != torch.int32 or t.shape != (n,) or t.device != device or not t.is_contiguous():
+    if t.dtype != _i32 or t.device != device or t.shape != (n,) or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 tensor [{n}] on the cache's device")
     return t.data_ptr()
 
 
 def _per_slot(name: str, t: torch.Tensor, cache: PagedKV, dtype: torch.dtype) -> int:
-    if t.dtype != dtype or tuple(t.shape) != cache.shape or t.device != cache.device or not t.is_contiguous():
+    if t.dtype != dtype or t.device != cache.device or t.shape != cache.shape or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {dtype} tensor [pages, kv heads, page_size] on the cache's device")
     return t.data_ptr()
 
@@ -168,23 +186,25 @@ def paged_append(cache: PagedKV, k: torch.Tensor, v: torch.Tensor, table: torch.
     rec_kv_append.  weights (fp32) and positions (int32), one value per slot:
     the written slots get 0 and their slot number."""
     dev = cache.device
-    t = _table(table, dev)
-    B, line = t.batch, (cache.shape[1], cache.head_dim)
-    for name, x in (("k", k), ("v", v)):
-        if x.dtype != cache.dtype or x.dim() != 3 or tuple(x.shape[1:]) != line or x.device != dev \
-                or x.stride(2) != 1 or x.stride(1) != line[1]:
-            raise ValueError(f"{name} must be {cache.dtype} [rows, {line[0]}, {line[1]}] on the cache's device, "
-                             "each row contiguous")
-    if k.shape[0] != v.shape[0]:
-        raise ValueError("k and v must have the same rows")
-    if k.shape[0] == 0:
+    t, B, _ = _table(table, dev)
+    heads, d, dtype = cache.shape[1], cache.head_dim, cache.dtype
+    rows, want = k.shape[0], (k.shape[0], heads, d)
+    (k0, k1, k2), (v0, v1, v2) = k.stride(), v.stride()
+    if k.dtype != dtype or v.dtype != dtype or k.shape != want or v.shape != want or k.device != dev \
+            or v.device != dev or k2 != 1 or v2 != 1 or (heads > 1 and (k1 != d or v1 != d)):
+        raise ValueError(f"k and v must be {dtype} [rows, {heads}, {d}] on the cache's device, each row contiguous")
+    if rows == 0:
         return
-    check(lib().rec_paged_append(
-        cache._ref, C.byref(t), k.data_ptr(), v.data_ptr(), k.stride(0), v.stride(0), k.shape[0],
+    if rows == 1:  # a single row's stride is never used
+        k0 = v0 = heads * d
+    code = lib().rec_paged_append(
+        cache._desc, t, k.data_ptr(), v.data_ptr(), k0, v0, rows,
         _ints("cu_seqlens", cu_seqlens, B + 1, dev), _ints("starts", starts, B, dev),
-        None if weights is None else _per_slot("weights", weights, cache, torch.float32),
-        None if positions is None else _per_slot("positions", positions, cache, torch.int32),
-        _status_ptr(dev), _stream(dev)), "rec_paged_append")
+        None if weights is None else _per_slot("weights", weights, cache, _f32),
+        None if positions is None else _per_slot("positions", positions, cache, _i32),
+        _status_ptr(cache._index), _stream(cache._index))
+    if code:
+        check(code, "rec_paged_append")
 
 
 def paged_attn_decode(cache: PagedKV, q: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, *,
@@ -203,46 +223,49 @@ def paged_attn_decode(cache: PagedKV, q: torch.Tensor, table: torch.Tensor, leng
     weights_out = decay * weights + the slot's softmax weights summed over the
     kv head's query heads, for every slot below the session's length;
     weights_out defaults to weights (in place)."""
-    dev = cache.device
-    t = _table(table, dev)
-    B, d = t.batch, cache.head_dim
-    if q.dtype != cache.dtype or q.dim() != 3 or q.shape[0] != B or q.shape[2] != d or q.device != dev \
+    dev, index, d = cache.device, cache._index, cache.head_dim
+    t, B, width = _table(table, dev)
+    shape = q.shape
+    if q.dtype != cache.dtype or len(shape) != 3 or shape[0] != B or shape[2] != d or q.device != dev \
             or q.stride(2) != 1:
         raise ValueError(f"q must be {cache.dtype} [{B}, query heads, {d}] on the cache's device, rows contiguous")
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    elif out.dtype != q.dtype or out.shape != q.shape or out.device != dev or out.stride(2) != 1:
+        out = torch.empty(shape, dtype=q.dtype, device=dev)
+    elif out.dtype != q.dtype or out.shape != shape or out.device != dev or out.stride(2) != 1:
         raise ValueError("out must match q, rows contiguous")
-    hq = q.shape[1]
-    a = abi.RecPagedAttn()
-    a.q, a.q_batch_stride, a.q_head_stride = q.data_ptr(), q.stride(0), q.stride(1)
-    a.out, a.out_batch_stride, a.out_head_stride = out.data_ptr(), out.stride(0), out.stride(1)
-    a.lengths = _ints("lengths", lengths, B, dev)
-    a.n_q_heads = hq
-    a.scale = d ** -0.5 if scale is None else scale
-    a.softcap, a.window = softcap, window
+    hq = shape[1]
+    lse_at = sinks_at = weights_at = weights_to = 0
     if lse is not None:
-        if lse.dtype != torch.float32 or lse.shape != (B, hq) or lse.device != dev or not lse.is_contiguous():
+        if lse.dtype != _f32 or lse.shape != (B, hq) or lse.device != dev or not lse.is_contiguous():
             raise ValueError(f"lse must be a contiguous fp32 tensor [{B}, {hq}] on the cache's device")
-        a.lse = lse.data_ptr()
+        lse_at = lse.data_ptr()
     if sinks is not None:
-        if sinks.dtype != torch.bfloat16 or sinks.shape != (hq,) or sinks.device != dev or not sinks.is_contiguous():
+        if sinks.dtype != _bf16 or sinks.shape != (hq,) or sinks.device != dev or not sinks.is_contiguous():
             raise ValueError(f"sinks must be a contiguous bf16 tensor [{hq}] on the cache's device")
-        a.sinks = sinks.data_ptr()
+        sinks_at = sinks.data_ptr()
     if weights is not None:
-        a.weights_in = _per_slot("weights", weights, cache, torch.float32)
-        a.weights_out = a.weights_in
+        weights_at = weights_to = _per_slot("weights", weights, cache, _f32)
+    else:
+        decay = 0.0
     if weights_out is not None:
-        a.weights_out = _per_slot("weights_out", weights_out, cache, torch.float32)
-    a.decay = decay if weights is not None else 0.0
-    tr = C.byref(t)
-    zero = C.c_size_t()
-    need = lib().rec_paged_attn_workspace_bytes(cache._ref, tr, hq, a.weights_out is not None, C.byref(zero))
-    stream = _stream(dev)
-    ws = _workspace("attn", dev, stream, max(need, 256))
-    counters = _workspace("attn counters", dev, stream, max(zero.value, 4096))  # every call leaves them zero
-    check(lib().rec_paged_attn_decode(cache._ref, tr, C.byref(a), ws.data_ptr(), ws.numel(), counters.data_ptr(),
-                                      counters.numel(), _status_ptr(dev), stream), "rec_paged_attn_decode")
+        weights_to = _per_slot("weights_out", weights_out, cache, _f32)
+    a = _ATTN.pack(q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1), lse_at,
+                   _ints("lengths", lengths, B, dev), sinks_at, hq, d ** -0.5 if scale is None else scale, softcap,
+                   window, weights_at, weights_to, decay)
+    L = lib()
+    key = (index, B, width, hq, d, cache.shape, cache.bits, weights_to != 0)
+    size = _sizes.get(key)
+    if size is None:
+        zero = C.c_size_t()
+        need = L.rec_paged_attn_workspace_bytes(cache._desc, t, hq, weights_to != 0, C.byref(zero))
+        size = (need, zero.value)
+        if need:
+            _sizes[key] = size
+    stream = _stream(index)
+    ws, ws_bytes, counters, counter_bytes = _buffers("attn", dev, index, stream, *size)
+    code = L.rec_paged_attn_decode(cache._desc, t, a, ws, ws_bytes, counters, counter_bytes, _status_ptr(index), stream)
+    if code:
+        check(code, "rec_paged_attn_decode")
     return out
 
 
@@ -264,28 +287,27 @@ def paged_evict(cache: PagedKV, table: torch.Tensor, lengths: torch.Tensor, budg
     counts as its own position.  weights_out and positions_out default to the
     inputs (in place).  The pages below the budget must not be shared with
     another session."""
-    dev = cache.device
-    t = _table(table, dev)
-    B = t.batch
+    dev, index = cache.device, cache._index
+    t, B, width = _table(table, dev)
     if lengths_out is None:
-        lengths_out = torch.empty(B, dtype=torch.int32, device=dev)
-    a = abi.RecPagedEvict()
-    a.lengths, a.lengths_out = _ints("lengths", lengths, B, dev), _ints("lengths_out", lengths_out, B, dev)
-    a.budget = budget
-    a.weights_in = _per_slot("weights", weights, cache, torch.float32)
-    a.weights_out = a.weights_in if weights_out is None else _per_slot("weights_out", weights_out, cache, torch.float32)
+        lengths_out = torch.empty(B, dtype=_i32, device=dev)
+    weights_at = weights_to = _per_slot("weights", weights, cache, _f32)
+    positions_at = positions_to = keep_at = 0
+    if weights_out is not None:
+        weights_to = _per_slot("weights_out", weights_out, cache, _f32)
     if positions is not None:
-        a.positions_in = _per_slot("positions", positions, cache, torch.int32)
-        a.positions_out = a.positions_in
+        positions_at = positions_to = _per_slot("positions", positions, cache, _i32)
     if positions_out is not None:
-        a.positions_out = _per_slot("positions_out", positions_out, cache, torch.int32)
+        positions_to = _per_slot("positions_out", positions_out, cache, _i32)
     if keep_from is not None:
-        a.keep_from = _ints("keep_from", keep_from, B, dev)
-    a.keep_below = keep_below
-    tr = C.byref(t)
-    need = lib().rec_paged_evict_workspace_bytes(cache._ref, tr, budget)
-    stream = _stream(dev)
-    ws = _workspace("evict", dev, stream, max(need, 256))
-    check(lib().rec_paged_evict(cache._ref, tr, C.byref(a), ws.data_ptr(), ws.numel(), _status_ptr(dev), stream),
-          "rec_paged_evict")
+        keep_at = _ints("keep_from", keep_from, B, dev)
+    a = _EVICT.pack(_ints("lengths", lengths, B, dev), _ints("lengths_out", lengths_out, B, dev), budget, weights_at,
+                    weights_to, positions_at, positions_to, keep_at, keep_below)
+    L = lib()
+    stream = _stream(index)
+    need = L.rec_paged_evict_workspace_bytes(cache._desc, t, budget)
+    ws, ws_bytes, _, _ = _buffers("evict", dev, index, stream, need, 0)
+    code = L.rec_paged_evict(cache._desc, t, a, ws, ws_bytes, _status_ptr(index), stream)
+    if code:
+        check(code, "rec_paged_evict")
     return lengths_out

@@ -10,12 +10,14 @@ ids bit for bit.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 import numpy as np
 import torch
 
 from . import abi
 from ._lib import check, lib
+from .ops import current_device as _current_device, raw_stream as _raw_stream
 
 
 def params(temperature=0.0, top_k=0, top_p=1.0, repetition_penalty=1.0, presence_penalty=0.0) -> abi.RecSampling:
@@ -188,15 +190,15 @@ def token_logprob(logits: torch.Tensor, p: abi.RecSampling, ids: torch.Tensor, h
 
 
 _LOGIT_TYPES = {torch.bfloat16: abi.REC_T_BF16, torch.float16: abi.REC_T_FP16, torch.float32: abi.REC_T_FP32}
+_RULES = struct.Struct("@Pi4x7Pi4xPq")  # abi.RecLogitRules as one pack
+assert _RULES.size == C.sizeof(abi.RecLogitRules)
 
 
-def _per_row(name: str, x, batch: int, dtype: torch.dtype, device) -> torch.Tensor | None:
-    """A contiguous [batch] tensor of `dtype` (a number is broadcast); None stays."""
-    if x is None:
-        return None
+def _per_row(name: str, x, batch: int, dtype: torch.dtype, device) -> torch.Tensor:
+    """A contiguous [batch] tensor of `dtype`; a number is broadcast."""
     if not isinstance(x, torch.Tensor):
         return torch.full((batch,), x, dtype=dtype, device=device)
-    if x.device != device or x.dtype != dtype or x.shape != (batch,) or not x.is_contiguous():
+    if x.dtype != dtype or x.shape != (batch,) or x.device != device or not x.is_contiguous():
         raise ValueError(f"{name} must be a number or a contiguous {dtype} tensor [{batch}] on the logits' device")
     return x
 
@@ -219,34 +221,37 @@ def process_logits(logits: torch.Tensor, history: torch.Tensor | None = None,
     allow: 32-bit words [B, W], W >= ceil(V / 32), bit i & 31 of word i >> 5
     set for each allowed id; the others get -inf.  `out` may be `logits`.
     sample_logits with the penalties off samples from the result."""
-    kind = _LOGIT_TYPES.get(logits.dtype)
-    if kind is None or not logits.is_cuda or logits.dim() != 2 or logits.stride(1) != 1:
+    kind, dev, shape = _LOGIT_TYPES.get(logits.dtype), logits.device, logits.shape
+    if kind is None or dev.type != "cuda" or len(shape) != 2 or logits.stride(1) != 1:
         raise ValueError("logits must be a bf16, fp16 or fp32 CUDA tensor [B, V] with contiguous rows")
-    B, V = logits.shape
-    dev = logits.device
-    if dev.index != torch.cuda.current_device():
+    B, V = shape
+    index = dev.index
+    if index != _current_device():
         raise ValueError("the tensors must live on the current CUDA device")
     if out is None:
-        out = torch.empty_like(logits, memory_format=torch.contiguous_format)
-    elif out.dtype != logits.dtype or out.shape != logits.shape or out.device != dev or out.stride(1) != 1:
+        out = torch.empty(shape, dtype=logits.dtype, device=dev)
+    elif out.dtype != logits.dtype or out.shape != shape or out.device != dev or out.stride(1) != 1:
         raise ValueError("out must match the logits, rows contiguous")
-    r = abi.RecLogitRules()
-    keep = []  # what a broadcast number became, until the launch
+    if B == 0 or V == 0:
+        return out
+    hist = cap = len_at = prompt_at = ids_at = values_at = m = allow_at = allow_stride = 0
+    rules = [None, None, None]  # kept until the launch
     if history is not None:
         if history.dtype != torch.int32 or history.dim() != 2 or history.shape[0] != B or history.device != dev \
                 or not history.is_contiguous():
             raise ValueError("history must be a contiguous int32 tensor [B, n] on the logits' device")
-        r.history_cap = history.shape[1]
-        if r.history_cap:
-            r.history = history.data_ptr()
+        cap = history.shape[1]
+        hist = history.data_ptr()
         if history_len is not None:
-            r.history_len = _per_row("history_len", history_len, B, torch.int32, dev).data_ptr()
+            len_at = _per_row("history_len", history_len, B, torch.int32, dev).data_ptr()
         if prompt_len is not None:
-            r.prompt_len = _per_row("prompt_len", prompt_len, B, torch.int32, dev).data_ptr()
-        for name, x in (("repetition", repetition), ("frequency", frequency), ("presence", presence)):
-            if x is not None:
-                keep.append(_per_row(name, x, B, torch.float32, dev))
-                setattr(r, name, keep[-1].data_ptr())
+            prompt_at = _per_row("prompt_len", prompt_len, B, torch.int32, dev).data_ptr()
+        if repetition is not None:
+            rules[0] = _per_row("repetition", repetition, B, torch.float32, dev)
+        if frequency is not None:
+            rules[1] = _per_row("frequency", frequency, B, torch.float32, dev)
+        if presence is not None:
+            rules[2] = _per_row("presence", presence, B, torch.float32, dev)
     elif history_len is not None or prompt_len is not None:
         raise ValueError("history_len and prompt_len need a history")
     if (bias_ids is None) != (bias_values is None):
@@ -256,17 +261,21 @@ def process_logits(logits: torch.Tensor, history: torch.Tensor | None = None,
                 or bias_ids.shape[0] != B or bias_values.shape != bias_ids.shape or bias_ids.device != dev \
                 or bias_values.device != dev or not bias_ids.is_contiguous() or not bias_values.is_contiguous():
             raise ValueError("bias_ids int32 and bias_values fp32 must be contiguous [B, m] on the logits' device")
-        r.n_bias = bias_ids.shape[1]
-        if r.n_bias:
-            r.bias_ids, r.bias_values = bias_ids.data_ptr(), bias_values.data_ptr()
+        m = bias_ids.shape[1]
+        ids_at, values_at = bias_ids.data_ptr(), bias_values.data_ptr()
     if allow is not None:
         if allow.element_size() != 4 or allow.dim() != 2 or allow.shape[0] != B or allow.device != dev \
                 or allow.stride(1) != 1 or allow.shape[1] < (V + 31) // 32:
             raise ValueError("allow must be 32-bit words [B, >= ceil(V / 32)] on the logits' device, rows contiguous")
-        r.allow, r.allow_stride = allow.data_ptr(), allow.stride(0)
-    if B:
-        check(lib().rec_process_logits(logits.data_ptr(), logits.stride(0), out.data_ptr(), out.stride(0), kind, B, V,
-                                       C.byref(r), torch.cuda.current_stream(dev).cuda_stream), "rec_process_logits")
+        allow_at, allow_stride = allow.data_ptr(), allow.stride(0)
+        if B == 1:
+            allow_stride = allow.shape[1]  # a single row's stride is never used
+    rep, freq, pres = (0 if x is None else x.data_ptr() for x in rules)
+    r = _RULES.pack(hist, cap, len_at, prompt_at, rep, freq, pres, ids_at, values_at, m, allow_at, allow_stride)
+    s_in, s_out = (logits.stride(0), out.stride(0)) if B > 1 else (V, V)
+    code = lib().rec_process_logits(logits.data_ptr(), s_in, out.data_ptr(), s_out, kind, B, V, r, _raw_stream(index))
+    if code:
+        check(code, "rec_process_logits")
     return out
 
 

@@ -140,3 +140,12 @@ def test_python_refuses_cpu_tensors():
         paged.PagedKV(x, x)
     with pytest.raises(ValueError):
         sampling.process_logits(torch.zeros(1, 10))
+
+
+def test_packs_match_the_structures():
+    def flat(t):
+        return [x for n, _ in t._fields_ for x in (getattr(t, n) if hasattr(getattr(t, n), "__len__") else [getattr(t, n)])]
+    for pack, kind, n in ((paged._KV, abi.RecPagedKV, 25), (paged._TABLE, abi.RecPagedTable, 4),
+                          (paged._ATTN, abi.RecPagedAttn, 16), (paged._EVICT, abi.RecPagedEvict, 9),
+                          (sampling._RULES, abi.RecLogitRules, 12)):
+        assert flat(kind.from_buffer_copy(pack.pack(*range(1, n + 1)))) == list(range(1, n + 1))
