@@ -30,8 +30,10 @@
 // the bias term then cancels little); q enters as fp16 after a power of two
 // that brings the head's largest value into [1, 2), so what fp16 loses is
 // below 2^-25 of it.  PV: p * scale_g is the P operand of group g (times a
-// power of two that follows the largest scale seen, in two fp16 parts) and
-// sum p * bias_g is added to the group's dims at the end.
+// power of two that follows the largest scale seen), rounded to fp16: a
+// relative 2^-12 per slot, a tenth of the output's own bf16 rounding, so its
+// low part is left out.  sum p * bias_g is added to the group's dims at the
+// end, in fp32.
 #pragma once
 #include "paged.cuh"
 
@@ -178,8 +180,7 @@ struct PagedSeg {
 template <class C>
 struct PagedTile {
   uint32_t k[C::TT][2][C::KW], v[C::TT][4][C::VW];
-  uint32_t ks[C::Q ? C::TT : 1][2][C::SW], kb[C::Q ? C::TT : 1][2][C::SW];
-  uint32_t vs[C::Q ? C::TT : 1][2][C::SW], vb[C::Q ? C::TT : 1][2][C::SW];
+  uint32_t ks[C::SW], kb[C::SW], vs[C::SW], vb[C::SW];  // codes: of the lane's own slot (0 past the end)
 };
 
 // Where a lane's slot of the coming tile is, in the pools' units.
@@ -192,15 +193,29 @@ template <int SW>
 __device__ __forceinline__ float scale_of(const uint32_t (&w)[SW], int g) {
   return g & 1 ? __uint_as_float(w[g >> 1] & 0xFFFF0000u) : __uint_as_float(w[g >> 1] << 16);
 }
+// A slot's scales and biases; 0 when it is not there.
 template <int NG, int SW>
-__device__ __forceinline__ void load_scales(uint32_t (&w)[SW], const uint16_t* p) {
-  if constexpr (NG == 1) w[0] = __ldg(p);
-  else if constexpr (NG == 2) w[0] = __ldg(reinterpret_cast<const unsigned*>(p));
-  else {
-    const uint2 x = __ldg(reinterpret_cast<const uint2*>(p));
-    w[0] = x.x;
-    w[1] = x.y;
+__device__ __forceinline__ void load_scales(uint32_t (&s)[SW], uint32_t (&b)[SW], const PagedScales& p, uint32_t at,
+                                            bool there) {
+#pragma unroll
+  for (int i = 0; i < SW; ++i) s[i] = b[i] = 0u;
+  if (!there) return;
+  if constexpr (NG == 1) {
+    s[0] = __ldg(p.s + at);
+    b[0] = __ldg(p.b + at);
+  } else if constexpr (NG == 2) {
+    s[0] = __ldg(reinterpret_cast<const unsigned*>(p.s + at));
+    b[0] = __ldg(reinterpret_cast<const unsigned*>(p.b + at));
+  } else {
+    const uint2 x = __ldg(reinterpret_cast<const uint2*>(p.s + at)), y = __ldg(reinterpret_cast<const uint2*>(p.b + at));
+    s[0] = x.x, s[1] = x.y, b[0] = y.x, b[1] = y.y;
   }
+}
+// The words of another lane's slot.
+template <int SW>
+__device__ __forceinline__ void from_lane(uint32_t (&d)[SW], const uint32_t (&w)[SW], int lane) {
+#pragma unroll
+  for (int i = 0; i < SW; ++i) d[i] = __shfl_sync(0xffffffffu, w[i], lane);
 }
 
 // Places of the TS slots from t0 of a segment (lane i: slot t0 + i % TS).
@@ -247,11 +262,9 @@ __device__ __forceinline__ void load_k(const PagedView& p, const PagedPlace& at,
         constexpr int n = C::KB == 8 ? 4 : 2;
 #pragma unroll
         for (int g = 0; g < C::NG; ++g) ldg_words<n>(&f.k[mt][r][n * g], row + 4 * n * (4 * g + q));
-        const size_t sc = __shfl_sync(0xffffffffu, at.ks, slot);
-        load_scales<C::NG>(f.ks[mt][r], p.ks.s + sc);
-        load_scales<C::NG>(f.kb[mt][r], p.ks.b + sc);
       }
     }
+  if constexpr (C::Q) load_scales<C::NG>(f.ks, f.kb, p.ks, at.ks, (at.valid >> (lane & (C::TS - 1))) & 1u);
 }
 
 template <class C>
@@ -274,14 +287,8 @@ __device__ __forceinline__ void load_v(const PagedView& p, const PagedPlace& at,
         }
       }
     }
-    if constexpr (C::Q)
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const size_t sc = __shfl_sync(0xffffffffu, at.vs, 16 * mt + 8 * r + j);
-        load_scales<C::NG>(f.vs[mt][r], p.vs.s + sc);
-        load_scales<C::NG>(f.vb[mt][r], p.vs.b + sc);
-      }
   }
+  if constexpr (C::Q) load_scales<C::NG>(f.vs, f.vb, p.vs, at.vs, (at.valid >> (lane & (C::TS - 1))) & 1u);
 }
 
 // The segment's queries into shared memory; codes: scaled fp16, group sums.
@@ -388,6 +395,14 @@ __device__ __forceinline__ void tile_scores(const PagedAttnArgs& a, const PagedS
         }
       }
   } else {
+    uint32_t ks[C::TT][2][C::SW], kb[C::TT][2][C::SW];
+#pragma unroll
+    for (int mt = 0; mt < C::TT; ++mt)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        from_lane(ks[mt][r], f.ks, 16 * mt + 8 * r + j);
+        from_lane(kb[mt][r], f.kb, 16 * mt + 8 * r + j);
+      }
 #pragma unroll
     for (int g = 0; g < C::NG; ++g) {
       float d[C::TT][C::NT][4];
@@ -433,7 +448,7 @@ __device__ __forceinline__ void tile_scores(const PagedAttnArgs& a, const PagedS
       for (int mt = 0; mt < C::TT; ++mt)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const float sc = scale_of(f.ks[mt][r], g), bi = __fmaf_rn(mid, sc, scale_of(f.kb[mt][r], g));
+          const float sc = scale_of(ks[mt][r], g), bi = __fmaf_rn(mid, sc, scale_of(kb[mt][r], g));
 #pragma unroll
           for (int nt = 0; nt < C::NT; ++nt)
 #pragma unroll
@@ -479,16 +494,15 @@ __device__ __forceinline__ void tile_fold(PagedTile<C>& f, uint32_t valid, float
         if (!((valid >> (16 * mt + 8 * r + j)) & 1u)) {
 #pragma unroll
           for (int nt = 0; nt < C::NT; ++nt) x[mt][nt][2 * r] = x[mt][nt][2 * r + 1] = -INFINITY;
-          if constexpr (C::Q)
-#pragma unroll
-            for (int i = 0; i < C::SW; ++i) f.vs[mt][r][i] = f.vb[mt][r][i] = 0u;
         }
-      if constexpr (!C::Q)
+      if constexpr (!C::Q) {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (!((valid >> (16 * mt + 2 * q + (e & 1) + 8 * (e >> 1))) & 1u))
+          if (!((valid >> (16 * mt + 2 * q + (e & 1) + 8 * (e >> 1))) & 1u)) {
 #pragma unroll
             for (int i = 0; i < C::VW; ++i) f.v[mt][e][i] = 0u;
+          }
+      }
     }
   }
   // the reference follows the maximum when it is passed by more than 8
@@ -507,11 +521,7 @@ __device__ __forceinline__ void tile_fold(PagedTile<C>& f, uint32_t valid, float
   float big = 0.0f;  // codes: the largest |scale|, in acc's units
   if constexpr (C::Q) {
 #pragma unroll
-    for (int mt = 0; mt < C::TT; ++mt)
-#pragma unroll
-      for (int r = 0; r < 2; ++r)
-#pragma unroll
-        for (int g = 0; g < C::NG; ++g) big = fmaxf(big, fabsf(scale_of(f.vs[mt][r], g)));
+    for (int g = 0; g < C::NG; ++g) big = fmaxf(big, fabsf(scale_of(f.vs, g)));
     move |= st.vf == 0.0f || big * st.vf > 64.0f;
   }
   if (__any_sync(0xffffffffu, move)) {
@@ -539,9 +549,10 @@ __device__ __forceinline__ void tile_fold(PagedTile<C>& f, uint32_t valid, float
         st.m[nt][e] = mn;
         st.mu[nt][e] = mu;
         st.l[nt][e] *= al;
-        if constexpr (C::Q)
+        if constexpr (C::Q) {
 #pragma unroll
           for (int g = 0; g < C::NG; ++g) st.xb[nt][e][g] *= al;
+        }
 #pragma unroll
         for (int g = 0; g < C::NG; ++g)
 #pragma unroll
@@ -563,24 +574,35 @@ __device__ __forceinline__ void tile_fold(PagedTile<C>& f, uint32_t valid, float
   // O^T += V^T P^T
 #pragma unroll
   for (int mt = 0; mt < C::TT; ++mt) {
-    uint32_t hi[C::NT][2], lo[C::NT][2];
+    uint32_t hi[C::NT][2], lo[C::NT][2];  // codes: hi alone
     auto split = [&](int nt, float w0, float w1, float w2, float w3) {
       const uint32_t h0 = pack16<C::F16>(w0, w1), h1 = pack16<C::F16>(w2, w3);
-      const float2 u0 = unpack16<C::F16>(h0), u1 = unpack16<C::F16>(h1);
       hi[nt][0] = trans8x8(h0);
       hi[nt][1] = trans8x8(h1);
-      lo[nt][0] = trans8x8(pack16<C::F16>(w0 - u0.x, w1 - u0.y));
-      lo[nt][1] = trans8x8(pack16<C::F16>(w2 - u1.x, w3 - u1.y));
+      if constexpr (!C::Q) {
+        const float2 u0 = unpack16<C::F16>(h0), u1 = unpack16<C::F16>(h1);
+        lo[nt][0] = trans8x8(pack16<C::F16>(w0 - u0.x, w1 - u0.y));
+        lo[nt][1] = trans8x8(pack16<C::F16>(w2 - u1.x, w3 - u1.y));
+      }
     };
-    if constexpr (!C::Q)
+    if constexpr (!C::Q) {
 #pragma unroll
       for (int nt = 0; nt < C::NT; ++nt) split(nt, x[mt][nt][0], x[mt][nt][1], x[mt][nt][2], x[mt][nt][3]);
+    }
+    uint32_t vs[2][C::SW], vb[2][C::SW];
+    if constexpr (C::Q) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        from_lane(vs[r], f.vs, 16 * mt + 8 * r + j);
+        from_lane(vb[r], f.vb, 16 * mt + 8 * r + j);
+      }
+    }
 #pragma unroll
     for (int g = 0; g < C::NG; ++g) {
       if constexpr (C::Q) {
         constexpr float mid = C::VB == 8 ? 128.0f : 8.0f;
-        const float s0 = scale_of(f.vs[mt][0], g), s1 = scale_of(f.vs[mt][1], g);
-        const float b0 = __fmaf_rn(mid, s0, scale_of(f.vb[mt][0], g)), b1 = __fmaf_rn(mid, s1, scale_of(f.vb[mt][1], g));
+        const float s0 = scale_of(vs[0], g), s1 = scale_of(vs[1], g);
+        const float b0 = __fmaf_rn(mid, s0, scale_of(vb[0], g)), b1 = __fmaf_rn(mid, s1, scale_of(vb[1], g));
         const float f0 = s0 * st.vf, f1 = s1 * st.vf;
 #pragma unroll
         for (int nt = 0; nt < C::NT; ++nt) {
@@ -624,7 +646,7 @@ __device__ __forceinline__ void tile_fold(PagedTile<C>& f, uint32_t valid, float
 #pragma unroll
         for (int nt = 0; nt < C::NT; ++nt) {
           mma16816<C::F16>(st.acc[nt][g][i], A[0], A[1], A[2], A[3], hi[nt][0], hi[nt][1]);
-          mma16816<C::F16>(st.acc[nt][g][i], A[0], A[1], A[2], A[3], lo[nt][0], lo[nt][1]);
+          if constexpr (!C::Q) mma16816<C::F16>(st.acc[nt][g][i], A[0], A[1], A[2], A[3], lo[nt][0], lo[nt][1]);
         }
       }
     }
@@ -780,9 +802,10 @@ __global__ void __launch_bounds__(C::W * 32, C::MINB) k_paged_attn(const PagedVi
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) {
           l += __shfl_xor_sync(0xffffffffu, l, o);
-          if constexpr (C::Q)
+          if constexpr (C::Q) {
 #pragma unroll
             for (int g = 0; g < C::NG; ++g) xb[g] += __shfl_xor_sync(0xffffffffu, xb[g], o);
+          }
         }
         if (j == 0) {
           sm.m[warp][n] = st.m[nt][e];
@@ -797,9 +820,10 @@ __global__ void __launch_bounds__(C::W * 32, C::MINB) k_paged_attn(const PagedVi
             y[2 * i] = st.acc[nt][g][i][e];
             y[2 * i + 1] = st.acc[nt][g][i][2 + e];
           }
-          if constexpr (C::Q)
+          if constexpr (C::Q) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) y[i] = __fmaf_rn(y[i], back, xb[g]);
+          }
           float4* dst = reinterpret_cast<float4*>(&sm.acc[warp][n][64 * g + 8 * j]);
           dst[0] = make_float4(y[0], y[1], y[2], y[3]);
           dst[1] = make_float4(y[4], y[5], y[6], y[7]);
@@ -857,18 +881,18 @@ __global__ void __launch_bounds__(C::W * 32, C::MINB) k_paged_attn(const PagedVi
     }
     if (!whole) {
       // the last of the head's blocks joins their partials, in block order
-      __threadfence();
       __syncthreads();
       const int c0 = int(head0 / per), c1 = int((head0 + s.nb - 1) / per), parts = c1 - c0 + 1;
       if (threadIdx.x == 0) {
         unsigned* c = a.counters + s.b * H + s.hh;
+        __threadfence();  // after the barrier: every thread's partial comes before the count
         const unsigned before = atomicAdd(c, 1u);
+        __threadfence();
         sm.last = before == unsigned(parts - 1);
         if (sm.last) *c = 0u;
       }
       __syncthreads();
       if (sm.last) {
-        __threadfence();
         float* wgt = &sm.acc[0][0][0];  // [HN][parts]
         auto part_slot = [&](int c) { return 2 * c + (int64_t(c) * per >= head0 ? 0 : 1); };
         for (int n = warp; n < heads; n += C::W) {
