@@ -17,15 +17,8 @@ struct QGroupParams {
   float scale, bias;
 };
 
-// All 32 lanes of a warp call this with the group's values v0 = w[2*lane],
-// v1 = w[2*lane+1].  Every lane returns the same parameters.
-__device__ __forceinline__ QGroupParams warp_group_params(float v0, float v1, int bits) {
-  float mx = fmaxf(v0, v1), mn = fminf(v0, v1);
-#pragma unroll
-  for (int off = 16; off >= 1; off >>= 1) {
-    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-    mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, off));
-  }
+// Parameters of a group with these extremes.
+__device__ __forceinline__ QGroupParams group_params(float mx, float mn, int bits) {
   const float n_bins = float((1 << bits) - 1);
   float scale = __fdiv_rn(__fsub_rn(mx, mn), n_bins);
   scale = scale > 1e-7f ? scale : 1e-7f;
@@ -39,6 +32,18 @@ __device__ __forceinline__ QGroupParams warp_group_params(float v0, float v1, in
     bias = edge;
   }
   return {scale, bias};
+}
+
+// All 32 lanes of a warp call this with the group's values v0 = w[2*lane],
+// v1 = w[2*lane+1].  Every lane returns the same parameters.
+__device__ __forceinline__ QGroupParams warp_group_params(float v0, float v1, int bits) {
+  float mx = fmaxf(v0, v1), mn = fminf(v0, v1);
+#pragma unroll
+  for (int off = 16; off >= 1; off >>= 1) {
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+    mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, off));
+  }
+  return group_params(mx, mn, bits);
 }
 
 __device__ __forceinline__ uint32_t quant_code(float w, QGroupParams p, int bits) {

@@ -326,6 +326,12 @@ def test_append_equals_the_single_session_append():
 
     heads, n, page = 2, 256, 64
     k, v = (torch.randn(n, heads, 128, device="cuda").bfloat16() for _ in range(2))
+    # quotients that lie on and beside halves
+    g = torch.Generator(device="cuda").manual_seed(1)
+    k[::2] = (torch.randint(-255, 256, k[::2].shape, device="cuda", generator=g).float() / 2).bfloat16()
+    v[::2] = (torch.randint(0, 511, v[::2].shape, device="cuda", generator=g).float() / 2).bfloat16()
+    v[::2, :, ::64] = 255.0
+    v[::2, :, 1::64] = 0.0
     flat = dict(k_codes=torch.zeros(heads, n, 32, dtype=torch.int32, device="cuda"))
     flat["v_codes"] = torch.zeros_like(flat["k_codes"])
     for name in ("k_scales", "k_biases", "v_scales", "v_biases"):
