@@ -1,14 +1,18 @@
 // Eviction from a paged cache by accumulated attention weight.
 //
-// Two kernels.  The first selects: a cluster of 1 to 8 blocks per (session,
-// kv head) holds the slots' rank keys in shared memory, finds the budget-th
-// largest by three radix passes (11, 11 and 10 bits; the blocks' histograms
-// meet in distributed shared memory), and lists the evicted slots below the
-// budget and the kept rows at or above it, each in slot order, as (page, row)
-// pairs.  The second moves row r of one list to place r of the other, one
-// 16-byte piece per thread.  Only holes are filled, so a cut of a few tokens
-// moves a few rows; sources are at or above the budget and places below it,
-// so no move reads what another wrote.
+// Two kernels, both bound by latency and by the scattered rows' sectors.  The
+// first selects: a cluster of 1 to 8 blocks per (session, kv head) holds the
+// slots' rank keys in shared memory, finds the budget-th largest by three
+// radix passes (11, 11 and 10 bits; the blocks' histograms meet in distributed
+// shared memory), and lists the evicted slots below the budget and the kept
+// slots at or above it, each in slot order.  A block takes up to 8,192 slots
+// (8 a thread) before a second one joins it: a pass over a cluster costs about
+// 2 us, eight more keys a thread far less.  The second kernel moves the r-th
+// kept row to the r-th hole: lane m of a warp finds the places of move m and
+// moves its scales, weight and position, then the warp moves the rows in
+// 16-byte pieces, four on their way per lane.  Only holes are filled, so a cut
+// of a few tokens moves a few rows; sources are at or above the budget and
+// places below it, so no move reads what another wrote.
 #include <limits.h>
 
 #include "cluster.cuh"
@@ -34,8 +38,7 @@ struct EvictArgs {
   int* p_out;
   const int* keep_from;
   int keep_below;
-  int2 *holes, *highs;  // [rows][cap] (page or -1, row of the page)
-  int* high_slot;       // [rows][cap]
+  int *holes, *highs;   // [rows][cap] slots
   int* counts;          // [rows]
   int cap;
   uint32_t* keys;       // [rows][slots] when a block's keys exceed its shared memory, or NULL
@@ -87,19 +90,24 @@ __global__ void __launch_bounds__(kThreads) k_evict_select(const PagedView p, co
     L = L < 0 ? 0 : int(p.slots);
   }
   const int budget = a.budget, kept = min(L, budget);
+  // slots that stay below the budget are copied when the outputs are other tensors; a hole's copy is
+  // overwritten by its move
   const bool copies = a.w_out != a.w_in || a.p_out != a.p_in;
-  auto copy_slot = [&](int t) {  // slot t stays where it is
-    int off;
-    const int page = slot_page(p, b, t, off);
-    if (page < 0) return;
-    const int64_t at = slot_index(p, page, h, off);
-    if (a.w_out != a.w_in) a.w_out[at] = a.w_in[at];
-    if (a.p_out && a.p_out != a.p_in) a.p_out[at] = a.p_in ? a.p_in[at] : t;
+  auto copy_slot = [&](int64_t at, int t, float w, int pos) {
+    if (t >= kept) return;
+    if (a.w_out != a.w_in) a.w_out[at] = w;
+    if (a.p_out && a.p_out != a.p_in) a.p_out[at] = pos;
   };
   if (L <= budget || budget == 0) {  // the same for the whole cluster
     if (rank == 0 && threadIdx.x == 0) a.counts[row] = 0;
     if (copies)
-      for (int t = rank * kThreads + threadIdx.x; t < kept; t += a.cluster * kThreads) copy_slot(t);
+      for (int t = rank * kThreads + threadIdx.x; t < kept; t += a.cluster * kThreads) {
+        int off;
+        const int page = slot_page(p, b, t, off);
+        if (page < 0) continue;
+        const int64_t at = slot_index(p, page, h, off);
+        copy_slot(at, t, a.w_in[at], a.p_in ? a.p_in[at] : t);
+      }
     return;
   }
   // this block's slots: [s0, s0 + n)
@@ -110,22 +118,38 @@ __global__ void __launch_bounds__(kThreads) k_evict_select(const PagedView p, co
   for (int i = threadIdx.x; i < 3 * kBins; i += kThreads) (&sm.hist[0][0])[i] = 0u;
   __syncthreads();
   const int from = a.keep_from ? a.keep_from[b] : INT_MAX;
-  for (int i0 = 0; i0 < n; i0 += kThreads) {
-    const int i = i0 + threadIdx.x;
-    uint32_t key = 0u;
-    if (i < n) {
+  constexpr int U = 8;  // slots of a thread on their way at once
+  for (int i0 = 0; i0 < n; i0 += U * kThreads) {
+    int64_t at[U];
+    float w[U];
+    int pos[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const int i = i0 + k * kThreads + int(threadIdx.x);
+      at[k] = -1;
+      if (i >= n) continue;
       int off;
-      const int t = s0 + i, page = slot_page(p, b, t, off);
-      if (page < 0) {
-        report(a.status, kStatusBadPage);
-      } else {
-        const int64_t at = slot_index(p, page, h, off);
-        const int pos = a.p_in ? a.p_in[at] : t;
-        key = rank_key(a.w_in[at], pos >= from || pos < a.keep_below);
-      }
-      keys[i] = key;
+      const int page = slot_page(p, b, s0 + i, off);
+      if (page < 0) report(a.status, kStatusBadPage);
+      else at[k] = slot_index(p, page, h, off);
     }
-    count_digit(sm.hist[0], key >> 21, i < n);
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      w[k] = at[k] >= 0 ? a.w_in[at[k]] : 0.0f;
+      pos[k] = at[k] >= 0 && a.p_in ? a.p_in[at[k]] : s0 + i0 + k * kThreads + int(threadIdx.x);
+    }
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const int i = i0 + k * kThreads + int(threadIdx.x);
+      if (i0 + k * kThreads >= n) break;  // for the whole block
+      uint32_t key = 0u;  // also of a slot whose page is bad
+      if (at[k] >= 0) {
+        key = rank_key(w[k], pos[k] >= from || pos[k] < a.keep_below);
+        if (copies) copy_slot(at[k], s0 + i, w[k], pos[k]);
+      }
+      if (i < n) keys[i] = key;
+      count_digit(sm.hist[0], key >> 21, i < n);
+    }
   }
   // the budget-th largest key T, and how many of its equals stay
   uint32_t T = 0;
@@ -145,11 +169,13 @@ __global__ void __launch_bounds__(kThreads) k_evict_select(const PagedView p, co
     // thread i sums bins 2(1023 - i) + 1 and 2(1023 - i): descending order
     const int d = 2 * (kThreads - 1 - int(threadIdx.x));
     int c1 = 0, c0 = 0;
-    for (int r = 0; r < a.cluster; ++r) {
-      const uint2 c = *reinterpret_cast<const uint2*>(peer(&sm.hist[pass][d], r));
-      c0 += int(c.x);
-      c1 += int(c.y);
-    }
+#pragma unroll
+    for (int r = 0; r < kMaxCluster; ++r)
+      if (r < a.cluster) {
+        const uint2 c = *reinterpret_cast<const uint2*>(peer(&sm.hist[pass][d], r));
+        c0 += int(c.x);
+        c1 += int(c.y);
+      }
     int x = c0 + c1;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -178,7 +204,13 @@ __global__ void __launch_bounds__(kThreads) k_evict_select(const PagedView p, co
   int tie0 = warps_before(ties, sm.scan, all);
   if (threadIdx.x == 0) sm.pub[0] = all;
   cluster_sync_all();
-  for (int r = 0; r < rank; ++r) tie0 += *peer(&sm.pub[0], r);
+  // lane r of every warp reads block r's count
+  auto of_peers = [&](int k, int& before) {
+    const int x = lane < a.cluster ? *peer(&sm.pub[k], lane) : 0;
+    before += __reduce_add_sync(0xffffffffu, lane < rank ? x : 0);
+    return __reduce_add_sync(0xffffffffu, x);
+  };
+  of_peers(0, tie0);
   const unsigned below = (1u << lane) - 1u;
   // keep / hole / survivor of the 32 slots from i0; tie counts on
   auto classify = [&](int i0, int& tie, bool& keep, bool& hole, bool& high) {
@@ -203,34 +235,18 @@ __global__ void __launch_bounds__(kThreads) k_evict_select(const PagedView p, co
   int high_at = warps_before(highs, sm.scan2, all);
   if (threadIdx.x == 0) sm.pub[2] = all;
   cluster_sync_all();
-  int moves = 0;
-  for (int r = 0; r < a.cluster; ++r) {
-    const int x = *peer(&sm.pub[1], r), y = *peer(&sm.pub[2], r);
-    moves += x;
-    if (r < rank) {
-      hole_at += x;
-      high_at += y;
-    }
-  }
+  const int moves = of_peers(1, hole_at);
+  of_peers(2, high_at);
   if (rank == 0 && threadIdx.x == 0) a.counts[row] = moves;
-  int2* hole_list = a.holes + int64_t(row) * a.cap;
-  int2* high_list = a.highs + int64_t(row) * a.cap;
-  int* slot_list = a.high_slot + int64_t(row) * a.cap;
+  int* hole_list = a.holes + int64_t(row) * a.cap;
+  int* high_list = a.highs + int64_t(row) * a.cap;
   tie = tie0;
   for (int i0 = i_lo; i0 < i_hi; i0 += 32) {
     bool keep, hole, high;
     classify(i0, tie, keep, hole, high);
     const unsigned ho = __ballot_sync(0xffffffffu, hole), hi = __ballot_sync(0xffffffffu, high);
-    const int t = s0 + i0 + lane;
-    if (hole || high) {
-      int off;
-      const int page = slot_page(p, b, t, off);
-      const int at = hole ? hole_at + __popc(ho & below) : high_at + __popc(hi & below);
-      (hole ? hole_list : high_list)[at] = make_int2(page, off);
-      if (high) slot_list[at] = t;
-    } else if (keep && copies) {
-      copy_slot(t);
-    }
+    if (hole) hole_list[hole_at + __popc(ho & below)] = s0 + i0 + lane;
+    if (high) high_list[high_at + __popc(hi & below)] = s0 + i0 + lane;
     hole_at += __popc(ho);
     high_at += __popc(hi);
   }
@@ -239,45 +255,82 @@ __global__ void __launch_bounds__(kThreads) k_evict_select(const PagedView p, co
 
 constexpr int kMoveThreads = 256;
 
-// Piece i of move m: the 16-byte pieces of K, of V, the scales and biases of
-// K and V (codes), then the weight and position.
+// A warp takes M moves at a time.
+template <int M>
 __global__ void __launch_bounds__(kMoveThreads) k_evict_move(const PagedView p, const EvictArgs a, const FastDiv per) {
   grid_wait();  // launched while the selection ends
-  const int row = blockIdx.y, b = row / p.hkv, h = row - b * p.hkv;
+  const int row = blockIdx.y, b = row / p.hkv, h = row - b * p.hkv, lane = threadIdx.x & 31;
   if (blockIdx.x == 0 && h == 0 && threadIdx.x == 0) {
     const int64_t L = max(0, a.lengths[b]);
     a.lengths_out[b] = int(min(min(L, p.slots), int64_t(a.budget)));
   }
   const int moves = a.counts[row];
-  const int2* hole_list = a.holes + int64_t(row) * a.cap;
-  const int2* high_list = a.highs + int64_t(row) * a.cap;
-  const int nk = p.d * p.k_bits / 128, nv = p.d * p.v_bits / 128;
-  const int groups = p.k_bits == 16 ? 0 : p.d / 64;
-  const int64_t pieces = int64_t(moves) * per.d;
-  const int step = gridDim.x * kMoveThreads;
-  for (int64_t x = int64_t(blockIdx.x) * kMoveThreads + threadIdx.x; x < pieces; x += step) {
-    const int m = x < INT_MAX ? int(fdiv(uint32_t(x), per)) : int(x / per.d);
-    int i = int(x - int64_t(m) * per.d);
-    const int2 to = hole_list[m], from = high_list[m];
-    if (to.x < 0 || from.x < 0) continue;
-    if (i < nk + nv) {
-      const PagedRows& r = i < nk ? p.k : p.v;
-      if (i >= nk) i -= nk;
-      reinterpret_cast<uint4*>(row_ptr(r, to.x, h, to.y))[i] =
-          reinterpret_cast<const uint4*>(row_ptr(r, from.x, h, from.y))[i];
-    } else if (i < int(per.d) - 1) {
-      i -= nk + nv;
-      const PagedScales& s = i < 2 ? p.ks : p.vs;
-      uint16_t* base = i & 1 ? s.b : s.s;
-      uint16_t* dst = base + scale_at(s, to.x, h, to.y);
-      const uint16_t* src = base + scale_at(s, from.x, h, from.y);
-      if (groups == 1) *dst = *src;
-      else if (groups == 2) *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(src);
-      else *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(src);
-    } else {
-      const int64_t dst = slot_index(p, to.x, h, to.y), src = slot_index(p, from.x, h, from.y);
-      a.w_out[dst] = a.w_in[src];
-      if (a.p_out) a.p_out[dst] = a.p_in ? a.p_in[src] : a.high_slot[int64_t(row) * a.cap + m];
+  const int* hole_list = a.holes + int64_t(row) * a.cap;
+  const int* high_list = a.highs + int64_t(row) * a.cap;
+  const int nk = p.d * p.k_bits / 128, groups = p.k_bits == 16 ? 0 : p.d / 64;
+  for (int m0 = (blockIdx.x * (kMoveThreads / 32) + (threadIdx.x >> 5)) * M; m0 < moves;
+       m0 += gridDim.x * (kMoveThreads / 32) * M) {
+    const int m = m0 + lane;
+    int page_to = -1, off_to = 0, page_from = -1, off_from = 0;
+    if (lane < M && m < moves) {
+      const int to = hole_list[m], from = high_list[m];
+      page_to = slot_page(p, b, to, off_to);
+      page_from = slot_page(p, b, from, off_from);
+      if (page_from < 0) page_to = -1;
+      if (page_to >= 0) {
+        const int64_t dst = slot_index(p, page_to, h, off_to), src = slot_index(p, page_from, h, off_from);
+        const float w = a.w_in[src];
+        const int pos = a.p_in ? a.p_in[src] : from;
+        if (groups) {
+          const size_t kd = scale_at(p.ks, page_to, h, off_to), kf = scale_at(p.ks, page_from, h, off_from);
+          const size_t vd = scale_at(p.vs, page_to, h, off_to), vf = scale_at(p.vs, page_from, h, off_from);
+          auto move4 = [&](auto* ks, auto* kb, auto* vs, auto* vb) {
+            const auto x = ks[0], y = kb[0];
+            const auto z = vs[0], u = vb[0];
+            using T = decltype(ks);
+            *reinterpret_cast<T>(p.ks.s + kd) = x;
+            *reinterpret_cast<T>(p.ks.b + kd) = y;
+            *reinterpret_cast<T>(p.vs.s + vd) = z;
+            *reinterpret_cast<T>(p.vs.b + vd) = u;
+          };
+          if (groups == 1) move4(p.ks.s + kf, p.ks.b + kf, p.vs.s + vf, p.vs.b + vf);
+          else if (groups == 2)
+            move4(reinterpret_cast<uint32_t*>(p.ks.s + kf), reinterpret_cast<uint32_t*>(p.ks.b + kf),
+                  reinterpret_cast<uint32_t*>(p.vs.s + vf), reinterpret_cast<uint32_t*>(p.vs.b + vf));
+          else
+            move4(reinterpret_cast<uint2*>(p.ks.s + kf), reinterpret_cast<uint2*>(p.ks.b + kf),
+                  reinterpret_cast<uint2*>(p.vs.s + vf), reinterpret_cast<uint2*>(p.vs.b + vf));
+        }
+        a.w_out[dst] = w;
+        if (a.p_out) a.p_out[dst] = pos;
+      }
+    }
+    // the rows' pieces: K's, then V's
+    const uint32_t k_to = page_to * p.k.page + h * p.k.head + off_to * p.k.row;
+    const uint32_t v_to = page_to * p.v.page + h * p.v.head + off_to * p.v.row;
+    const uint32_t k_from = page_from * p.k.page + h * p.k.head + off_from * p.k.row;
+    const uint32_t v_from = page_from * p.v.page + h * p.v.head + off_from * p.v.row;
+    const int pieces = min(M, moves - m0) * int(per.d);
+    constexpr int U = 4;
+    for (int x0 = 0; x0 < pieces; x0 += 32 * U) {
+      uint4 val[U];
+      uint8_t* dst[U];
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        const int x = x0 + 32 * i + lane;
+        const int mm = min(int(fdiv(x, per)), M - 1), e = x - int(fdiv(x, per)) * int(per.d);
+        const bool there = __shfl_sync(0xffffffffu, page_to, mm) >= 0 && x < pieces;
+        const uint32_t kt = __shfl_sync(0xffffffffu, k_to, mm), kf = __shfl_sync(0xffffffffu, k_from, mm);
+        const uint32_t vt = __shfl_sync(0xffffffffu, v_to, mm), vf = __shfl_sync(0xffffffffu, v_from, mm);
+        const bool is_k = e < nk;
+        const size_t piece = size_t(is_k ? e : e - nk);
+        dst[i] = there ? (is_k ? p.k.base : p.v.base) + ((size_t(is_k ? kt : vt) + piece) << 4) : nullptr;
+        if (there)
+          val[i] = __ldcs(reinterpret_cast<const uint4*>((is_k ? p.k.base : p.v.base) + ((size_t(is_k ? kf : vf) + piece) << 4)));
+      }
+#pragma unroll
+      for (int i = 0; i < U; ++i)
+        if (dst[i]) *reinterpret_cast<uint4*>(dst[i]) = val[i];
     }
   }
 }
@@ -285,24 +338,25 @@ __global__ void __launch_bounds__(kMoveThreads) k_evict_move(const PagedView p, 
 struct EvictLayout {
   int cluster, cap;
   bool shared;  // the keys fit shared memory
-  size_t holes, highs, slots, counts, keys, total;
+  size_t holes, highs, counts, keys, total;
 };
 EvictLayout evict_layout(int64_t slots, int batch, int hkv, int budget) {
   EvictLayout l;
   const int64_t rows = int64_t(batch) * hkv;
   auto slice = [&](int c) { return ((slots + c - 1) / c + 31) / 32 * 32; };
-  // more blocks per row while the rows leave SMs idle and a block has more than 1,024 keys
+  // more blocks per row while a block has more than 8,192 keys and every block has an SM (one block
+  // fills it: 8 sessions x 4 heads of 65,536 slots take 47 us in clusters of 4, 87 us in two waves of
+  // clusters of 8), or while the keys do not fit
   l.cluster = 1;
   while (l.cluster < kMaxCluster && (slice(l.cluster) > kKeysInShared ||
-                                     (rows * l.cluster < 148 && slice(l.cluster) > 1024)))
+                                     (slice(l.cluster) > 8192 && rows * l.cluster * 2 <= sm_count())))
     l.cluster *= 2;
   l.shared = slice(l.cluster) <= kKeysInShared;
   l.cap = int(slots < budget ? slots : budget);
   auto up = [](size_t n) { return (n + 255) / 256 * 256; };
   l.holes = 0;
-  l.highs = up(size_t(rows) * l.cap * 8);
-  l.slots = 2 * l.highs;
-  l.counts = l.slots + up(size_t(rows) * l.cap * 4);
+  l.highs = up(size_t(rows) * l.cap * 4);
+  l.counts = 2 * l.highs;
   l.keys = l.counts + up(size_t(rows) * 4);
   l.total = l.keys + (l.shared ? 0 : up(size_t(rows) * size_t(slots) * 4));
   return l;
@@ -342,9 +396,8 @@ REC_API int rec_paged_evict(const RecPagedKV* kv, const RecPagedTable* table, co
   a.p_out = evict->positions_out;
   a.keep_from = evict->keep_from;
   a.keep_below = evict->keep_below;
-  a.holes = reinterpret_cast<int2*>(ws + l.holes);
-  a.highs = reinterpret_cast<int2*>(ws + l.highs);
-  a.high_slot = reinterpret_cast<int*>(ws + l.slots);
+  a.holes = reinterpret_cast<int*>(ws + l.holes);
+  a.highs = reinterpret_cast<int*>(ws + l.highs);
   a.counts = reinterpret_cast<int*>(ws + l.counts);
   a.cap = l.cap;
   a.keys = l.shared ? nullptr : reinterpret_cast<uint32_t*>(ws + l.keys);
@@ -365,11 +418,14 @@ REC_API int rec_paged_evict(const RecPagedKV* kv, const RecPagedTable* table, co
   REC_CHECK_CUDA(set_smem_limit(reinterpret_cast<const void*>(&k_evict_select),
                                 sizeof(SelectSmem) + size_t(kKeysInShared) * 4));
   REC_CHECK_CUDA(cudaLaunchKernelEx(&cfg, k_evict_select, p, a));
-  const unsigned per = unsigned(p.d * (p.k_bits + p.v_bits) / 128 + (p.k_bits == 16 ? 0 : 4) + 1);
-  // blocks per row: two waves of the SMs over all rows, no more than a full list needs
-  const int64_t most = (int64_t(l.cap) * per + kMoveThreads - 1) / kMoveThreads;
-  int64_t x = (int64_t(sm_count()) * 16 + rows - 1) / rows;
-  x = x < most ? x : most;
+  const FastDiv per = make_fastdiv(unsigned(p.d * (p.k_bits + p.v_bits) / 128));
+  // moves of a row: no more than the budget, nor than the slots above it.  32 a warp; 8 where that
+  // leaves SMs idle
+  const int64_t most = p.slots > a.budget ? (p.slots - a.budget < l.cap ? p.slots - a.budget : l.cap) : 0;
+  const int batch = most * rows >= int64_t(sm_count()) * 32 * 32 ? 32 : 8;
+  const int64_t full = (most + 8 * batch - 1) / (8 * batch);  // blocks of 8 warps for a row's most moves
+  int64_t x = (int64_t(sm_count()) * 8 + rows - 1) / rows;
+  x = x < full ? x : full;
   cudaLaunchConfig_t mv = {};
   mv.gridDim = dim3(unsigned(x < 1 ? 1 : x), rows);
   mv.blockDim = dim3(kMoveThreads);
@@ -378,6 +434,7 @@ REC_API int rec_paged_evict(const RecPagedKV* kv, const RecPagedTable* table, co
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   mv.attrs = attr;
   mv.numAttrs = 1;
-  REC_CHECK_CUDA(cudaLaunchKernelEx(&mv, k_evict_move, p, a, make_fastdiv(per)));
+  if (batch == 32) REC_CHECK_CUDA(cudaLaunchKernelEx(&mv, k_evict_move<32>, p, a, per));
+  else REC_CHECK_CUDA(cudaLaunchKernelEx(&mv, k_evict_move<8>, p, a, per));
   return REC_OK;
 }
