@@ -1,15 +1,17 @@
 // Per-row rules on a batch of logits: repetition, frequency and presence
 // penalties by a row's own history, biases, an allow mask (rec_process_logits).
 //
-// One block per (row, chunk of the vocabulary).  Every thread first asks for
-// its logits (16-byte pieces, all of them on their way before anything else);
-// meanwhile the block marks, in one shared word per id, what the row's lists
-// say of the ids of its chunk: bits 0-17 the id's count after the prompt, bits
-// 18-30 one more than the last bias entry that names it, bit 31 whether the
-// history has it at all.  A piece whose words are all 0 is copied, with the
-// masked ids replaced; the others go through fp32.  The lists are read once
-// per chunk (from L2 after the first), so the chunk is the largest that keeps
-// the SMs busy, up to 8,192 ids (32 KB of words, 4 blocks an SM).
+// One block per (row, chunk of the vocabulary).  The logits stream through in
+// 16-byte pieces, all of a thread's asked for before anything else, and only
+// the mask touches them on the way; meanwhile the block marks, in one shared
+// word per id, what the row's lists say of the ids of its chunk: bits 0-17 the
+// id's count after the prompt, bits 18-30 one more than the last bias entry
+// that names it, bit 31 whether the history has it at all.  The ids that get a
+// word are listed once, and after the stream one thread each rewrites them: a
+// history names a few percent of the ids, and looking for them in every piece
+// would send every warp through the divisions.  The lists are read once per
+// chunk (from L2 after the first), so the chunk is the largest that keeps the
+// SMs busy, up to 8,192 ids.
 #include "capi_common.h"
 #include "common.cuh"
 
@@ -62,12 +64,14 @@ __device__ __forceinline__ float apply(float x, unsigned w, const RowRules& r) {
 }
 
 template <int T>
-__global__ void __launch_bounds__(kThreads) k_process_logits(const LogitArgs a) {
+__global__ void __launch_bounds__(kThreads, 4) k_process_logits(const LogitArgs a) {
   using L = LogitType<T>;
   using raw = typename L::raw;
   constexpr int E = 16 / sizeof(raw);                 // ids of a piece
   constexpr int N = kMaxChunk / E / kThreads;         // pieces of a thread
-  __shared__ __align__(16) unsigned word[kMaxChunk];
+  extern __shared__ __align__(16) unsigned word[];  // [chunk]
+  uint16_t* listed = reinterpret_cast<uint16_t*>(word + a.chunk);
+  __shared__ int n_listed;
   const int b = blockIdx.y;
   const RecLogitRules& r = a.r;
   const raw* in = static_cast<const raw*>(a.in) + b * a.stride;
@@ -86,14 +90,55 @@ __global__ void __launch_bounds__(kThreads) k_process_logits(const LogitArgs a) 
       if (i + E <= n && first + i >= 0) x[k] = __ldcs(reinterpret_cast<const uint4*>(in + first + i));
     }
   }
-  for (int i = 4 * threadIdx.x; i < n; i += 4 * kThreads) *reinterpret_cast<uint4*>(&word[i]) = make_uint4(0u, 0u, 0u, 0u);
+  const bool lists = r.n_bias || r.history_cap;
+  if (lists) {
+    if (threadIdx.x == 0) n_listed = 0;
+    for (int i = 4 * threadIdx.x; i < n; i += 4 * kThreads)
+      *reinterpret_cast<uint4*>(&word[i]) = make_uint4(0u, 0u, 0u, 0u);
+  }
+  const uint32_t* allow = r.allow ? r.allow + b * r.allow_stride : nullptr;
+  auto allowed = [&](int id) { return !allow || ((__ldg(allow + (id >> 5)) >> (id & 31)) & 1u); };
+  if (wide) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int i = (k * kThreads + threadIdx.x) * E;
+      if (i >= n) break;
+      if (i + E > n || first + i < 0) {  // the row's ends
+        for (int e = 0; e < E && i + e < n; ++e)
+          if (first + i + e >= 0) out[first + i + e] = allowed(first + i + e) ? in[first + i + e] : L::low;
+        continue;
+      }
+      if (allow) {
+        const int id = first + i, q = id >> 5, s = id & 31;
+        const uint32_t lo = __ldg(allow + q), hi = s + E > 32 ? __ldg(allow + q + 1) : 0u;
+        const unsigned bits = __funnelshift_r(lo, hi, s);
+        uint32_t* y = reinterpret_cast<uint32_t*>(&x[k]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if constexpr (E == 4) {
+            y[j] = (bits >> j) & 1u ? y[j] : L::low;
+          } else {  // all ones in the halves that stay
+            const uint32_t m = ((bits >> (2 * j)) & 1u) * 0xFFFFu | ((bits >> (2 * j + 1)) & 1u) * 0xFFFF0000u;
+            y[j] = (y[j] & m) | ((uint32_t(L::low) * 0x10001u) & ~m);
+          }
+        }
+      }
+      *reinterpret_cast<uint4*>(out + first + i) = x[k];
+    }
+  } else {
+    for (int i = threadIdx.x; i < n; i += kThreads)
+      if (first + i >= 0) out[first + i] = allowed(first + i) ? in[first + i] : L::low;
+  }
+  if (!lists) return;
   __syncthreads();
-  const RowRules rules = {r.repetition ? __ldg(r.repetition + b) : 1.0f, r.frequency ? __ldg(r.frequency + b) : 0.0f,
-                          r.presence ? __ldg(r.presence + b) : 0.0f, r.bias_values + int64_t(b) * r.n_bias};
+  auto list = [&](int i, unsigned before) {
+    if (before == 0u) listed[atomicAdd(&n_listed, 1)] = uint16_t(i);
+  };
   if (r.n_bias) {
     for (int j = threadIdx.x; j < r.n_bias; j += kThreads) {
       const int id = __ldg(r.bias_ids + int64_t(b) * r.n_bias + j);
-      if (id >= 0 && id < a.V && unsigned(id - first) < unsigned(n)) atomicMax(&word[id - first], unsigned(j + 1) << 18);
+      if (id >= 0 && id < a.V && unsigned(id - first) < unsigned(n))
+        list(id - first, atomicMax(&word[id - first], unsigned(j + 1) << 18));
     }
     __syncthreads();
   }
@@ -101,72 +146,40 @@ __global__ void __launch_bounds__(kThreads) k_process_logits(const LogitArgs a) 
     const int len = min(r.history_cap, r.history_len ? max(0, __ldg(r.history_len + b)) : r.history_cap);
     const int prompt = r.prompt_len ? __ldg(r.prompt_len + b) : 0;
     const int* hist = r.history + int64_t(b) * r.history_cap;
-#pragma unroll 4
+    // the ids that count for this chunk: [max(first, 0), first + n), and first + n <= V
+    const unsigned lo = unsigned(max(first, 0)), span = unsigned(first + n) - lo;
+#pragma unroll 8
     for (int j = threadIdx.x; j < len; j += kThreads) {
-      const int id = __ldg(hist + j);
-      if (id < 0 || id >= a.V || unsigned(id - first) >= unsigned(n)) continue;
+      const unsigned id = unsigned(__ldg(hist + j));
+      if (id - lo >= span) continue;
+      const int i = int(id) - first;
       if (j < prompt) {
-        atomicOr(&word[id - first], 0x80000000u);
-      } else if (!((atomicAdd(&word[id - first], 1u)) >> 31)) {
-        atomicOr(&word[id - first], 0x80000000u);
+        list(i, atomicOr(&word[i], 0x80000000u));
+      } else {
+        const unsigned before = atomicAdd(&word[i], 1u);
+        if (!(before >> 31)) atomicOr(&word[i], 0x80000000u);
+        list(i, before);
       }
     }
     __syncthreads();
   }
-  const uint32_t* allow = r.allow ? r.allow + b * r.allow_stride : nullptr;
-  auto one = [&](int i) {  // id first + i on its own
-    const int id = first + i;
-    if (id < 0) return;
-    raw y = in[id];
-    const unsigned w = word[i];
-    if (w) y = L::put(apply(L::get(y), w, rules));
-    if (allow && !((__ldg(allow + (id >> 5)) >> (id & 31)) & 1u)) y = L::low;
-    out[id] = y;
-  };
-  if (!wide) {
-    for (int i = threadIdx.x; i < n; i += kThreads) one(i);
-    return;
-  }
-#pragma unroll
-  for (int k = 0; k < N; ++k) {
-    const int i = (k * kThreads + threadIdx.x) * E;
-    if (i >= n) break;
-    if (i + E > n || first + i < 0) {
-      for (int e = 0; e < E && i + e < n; ++e) one(i + e);
-      continue;
-    }
-    unsigned w[E], any = 0u;
-#pragma unroll
-    for (int e = 0; e < E; e += 4) {
-      const uint4 v = *reinterpret_cast<const uint4*>(&word[i + e]);
-      w[e] = v.x, w[e + 1] = v.y, w[e + 2] = v.z, w[e + 3] = v.w;
-      any |= v.x | v.y | v.z | v.w;
-    }
-    unsigned bits = (1u << E) - 1u;
-    if (allow) {
-      const int id = first + i, q = id >> 5, s = id & 31;
-      const uint32_t lo = __ldg(allow + q), hi = s + E > 32 ? __ldg(allow + q + 1) : 0u;
-      bits &= __funnelshift_r(lo, hi, s);
-    }
-    if (any || bits != (1u << E) - 1u) {
-      raw y[E];
-      *reinterpret_cast<uint4*>(y) = x[k];
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        if (w[e]) y[e] = L::put(apply(L::get(y[e]), w[e], rules));
-        if (!((bits >> e) & 1u)) y[e] = L::low;
-      }
-      x[k] = *reinterpret_cast<uint4*>(y);
-    }
-    __stcs(reinterpret_cast<uint4*>(out + first + i), x[k]);
+  const RowRules rules = {r.repetition ? __ldg(r.repetition + b) : 1.0f, r.frequency ? __ldg(r.frequency + b) : 0.0f,
+                          r.presence ? __ldg(r.presence + b) : 0.0f, r.bias_values + int64_t(b) * r.n_bias};
+  for (int k = threadIdx.x; k < n_listed; k += kThreads) {
+    const int i = listed[k], id = first + i;
+    // in place, a masked id reads as -inf here and stays that
+    if (allowed(id)) out[id] = L::put(apply(L::get(in[id]), word[i], rules));
   }
 }
 
 template <int T>
-void launch(const LogitArgs& a, int batch, cudaStream_t st) {
+cudaError_t launch(const LogitArgs& a, int batch, cudaStream_t st) {
+  const cudaError_t e = set_smem_limit(reinterpret_cast<const void*>(&k_process_logits<T>), kMaxChunk * 6);
+  if (e != cudaSuccess) return e;
   constexpr int E = 16 / int(sizeof(typename LogitType<T>::raw));
   const int64_t span = int64_t(a.V) + E - 1;  // with the row's skew
-  k_process_logits<T><<<dim3(unsigned((span + a.chunk - 1) / a.chunk), batch), kThreads, 0, st>>>(a);
+  k_process_logits<T><<<dim3(unsigned((span + a.chunk - 1) / a.chunk), batch), kThreads, a.chunk * 6, st>>>(a);
+  return cudaGetLastError();
 }
 
 }  // namespace
@@ -192,9 +205,8 @@ REC_API int rec_process_logits(const void* logits, int64_t stride, void* logits_
   // small batches: chunks of at least 1,024 ids until every SM has a block
   while (a.chunk > 1024 && int64_t(batch) * ((vocab + a.chunk - 1) / a.chunk) < sm_count()) a.chunk /= 2;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (dtype == REC_T_FP32) launch<REC_T_FP32>(a, batch, st);
-  else if (dtype == REC_T_BF16) launch<REC_T_BF16>(a, batch, st);
-  else launch<REC_T_FP16>(a, batch, st);
-  REC_CHECK_CUDA(cudaGetLastError());
+  if (dtype == REC_T_FP32) REC_CHECK_CUDA(launch<REC_T_FP32>(a, batch, st));
+  else if (dtype == REC_T_BF16) REC_CHECK_CUDA(launch<REC_T_BF16>(a, batch, st));
+  else REC_CHECK_CUDA(launch<REC_T_FP16>(a, batch, st));
   return REC_OK;
 }
