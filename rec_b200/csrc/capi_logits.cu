@@ -6,12 +6,12 @@
 // the mask touches them on the way; meanwhile the block marks, in one shared
 // word per id, what the row's lists say of the ids of its chunk: bits 0-17 the
 // id's count after the prompt, bits 18-30 one more than the last bias entry
-// that names it, bit 31 whether the history has it at all.  The ids that get a
+// that names it, bit 31 whether the prompt has it.  The ids that get a
 // word are listed once, and after the stream one thread each rewrites them: a
 // history names a few percent of the ids, and looking for them in every piece
 // would send every warp through the divisions.  The lists are read once per
-// chunk (from L2 after the first), so the chunk is the largest that keeps the
-// SMs busy, up to 8,192 ids.
+// chunk (from L2 after the first), so the chunks are as few as fill whole
+// waves of blocks, up to 9,216 ids each.
 #include "capi_common.h"
 #include "common.cuh"
 
@@ -20,7 +20,7 @@ using namespace rec;
 namespace {
 
 constexpr int kThreads = 512;
-constexpr int kMaxChunk = 8192;
+constexpr int kMaxChunk = 9216;  // 54 KB of words and places: 4 blocks an SM
 constexpr int kMaxHistory = (1 << 18) - 1;
 constexpr int kMaxBias = (1 << 13) - 2;
 
@@ -55,8 +55,8 @@ struct RowRules {
 };
 // The penalties and the bias that an id's word w asks for.
 __device__ __forceinline__ float apply(float x, unsigned w, const RowRules& r) {
-  if (w >> 31) x = x < 0.0f ? __fmul_rn(x, r.rho) : __fdiv_rn(x, r.rho);
   const unsigned c = w & 0x3FFFFu;
+  if (c || w >> 31) x = x < 0.0f ? __fmul_rn(x, r.rho) : __fdiv_rn(x, r.rho);
   if (c) x = __fsub_rn(__fsub_rn(x, __fmul_rn(r.freq, float(c))), r.pres);
   const unsigned m = (w >> 18) & 0x1FFFu;
   if (m) x = __fadd_rn(x, r.bias[m - 1]);
@@ -68,18 +68,18 @@ __global__ void __launch_bounds__(kThreads, 4) k_process_logits(const LogitArgs 
   using L = LogitType<T>;
   using raw = typename L::raw;
   constexpr int E = 16 / sizeof(raw);                 // ids of a piece
-  constexpr int N = kMaxChunk / E / kThreads;         // pieces of a thread
+  constexpr int N = (kMaxChunk / E + kThreads - 1) / kThreads;  // pieces of a thread
   extern __shared__ __align__(16) unsigned word[];  // [chunk]
   uint16_t* listed = reinterpret_cast<uint16_t*>(word + a.chunk);
   __shared__ int n_listed;
-  const int b = blockIdx.y;
+  const int b = blockIdx.x;
   const RecLogitRules& r = a.r;
   const raw* in = static_cast<const raw*>(a.in) + b * a.stride;
   raw* out = static_cast<raw*>(a.out) + b * a.out_stride;
   // ids before the first 16-byte boundary of the row; the chunks start there
   const int skew = int((reinterpret_cast<uintptr_t>(in) & 15u) / sizeof(raw));
   const bool wide = skew == int((reinterpret_cast<uintptr_t>(out) & 15u) / sizeof(raw));
-  const int first = blockIdx.x * a.chunk - (wide ? skew : 0);  // id of word 0; below 0 at most in the first piece
+  const int first = blockIdx.y * a.chunk - (wide ? skew : 0);  // id of word 0; below 0 at most in the first piece
   const int n = min(a.chunk, a.V - first);
   if (n <= 0) return;
   uint4 x[N];
@@ -153,13 +153,7 @@ __global__ void __launch_bounds__(kThreads, 4) k_process_logits(const LogitArgs 
       const unsigned id = unsigned(__ldg(hist + j));
       if (id - lo >= span) continue;
       const int i = int(id) - first;
-      if (j < prompt) {
-        list(i, atomicOr(&word[i], 0x80000000u));
-      } else {
-        const unsigned before = atomicAdd(&word[i], 1u);
-        if (!(before >> 31)) atomicOr(&word[i], 0x80000000u);
-        list(i, before);
-      }
+      list(i, j < prompt ? atomicOr(&word[i], 0x80000000u) : atomicAdd(&word[i], 1u));
     }
     __syncthreads();
   }
@@ -178,7 +172,7 @@ cudaError_t launch(const LogitArgs& a, int batch, cudaStream_t st) {
   if (e != cudaSuccess) return e;
   constexpr int E = 16 / int(sizeof(typename LogitType<T>::raw));
   const int64_t span = int64_t(a.V) + E - 1;  // with the row's skew
-  k_process_logits<T><<<dim3(unsigned((span + a.chunk - 1) / a.chunk), batch), kThreads, a.chunk * 6, st>>>(a);
+  k_process_logits<T><<<dim3(batch, unsigned((span + a.chunk - 1) / a.chunk)), kThreads, a.chunk * 6, st>>>(a);
   return cudaGetLastError();
 }
 
@@ -202,8 +196,12 @@ REC_API int rec_process_logits(const void* logits, int64_t stride, void* logits_
                 "rec_process_logits: %d bias entries (at most %d)", r.n_bias, kMaxBias);
   REC_CHECK_ARG(!r.allow || r.allow_stride >= (vocab + 31) / 32, "rec_process_logits: allow rows too short");
   LogitArgs a = {logits, logits_out, stride, out_stride, vocab, kMaxChunk, r};
-  // small batches: chunks of at least 1,024 ids until every SM has a block
-  while (a.chunk > 1024 && int64_t(batch) * ((vocab + a.chunk - 1) / a.chunk) < sm_count()) a.chunk /= 2;
+  // whole waves of blocks, and at least 1,024 ids a block
+  const int64_t wave = int64_t(sm_count()) * 4, span = int64_t(vocab) + 7;
+  const int64_t waves = (batch * ((span + kMaxChunk - 1) / kMaxChunk) + wave - 1) / wave;
+  const int64_t chunks = wave * waves / batch;  // at least span / kMaxChunk of them
+  const int64_t chunk = ((span + chunks - 1) / chunks + 15) / 16 * 16;
+  a.chunk = int(chunk < 1024 ? 1024 : chunk < kMaxChunk ? chunk : kMaxChunk);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == REC_T_FP32) REC_CHECK_CUDA(launch<REC_T_FP32>(a, batch, st));
   else if (dtype == REC_T_BF16) REC_CHECK_CUDA(launch<REC_T_BF16>(a, batch, st));
