@@ -16,7 +16,15 @@
 // into the registers that the MMA reads: no shared memory, no transposition
 // for K, and one byte permutation per register for V (two slots of one dim
 // into a pair).  K of the next tile is on its way while this tile's softmax
-// and PV run, V while the next scores run.
+// and PV run, V while the next scores run; where every block has more than 16
+// tiles a warp, 16-bit rows are also asked for in L2 a tile earlier (64 sessions
+// up to 16K: 188 -> 181 us; over ten tiles a warp it costs more than it brings,
+// 45.4 -> 47.5 us, and so it does for codes, whose widening takes as many
+// instructions again).  All blocks or none: asking in long segments only
+// starved the blocks with short ones (220 us), and without the next segment's
+// first tiles nothing is gained.
+// Loads on their way hold L1 space, so shared memory is kept small: 227 KB of
+// it instead of 54 took the same case from 188 to 241 us.
 //
 // Softmax.  s in log2 units; m is a reference per head that follows the
 // running maximum when it is passed by more than 8 (p <= 256 until then), so
@@ -241,6 +249,27 @@ __device__ __forceinline__ void find_places(const PagedView& p, const PagedAttnA
     at.vs = page * p.vs.page + s.h * p.vs.head + off * p.vs.row;
   }
   at.valid = __ballot_sync(0xffffffffu, ok) & (C::TS == 32 ? 0xffffffffu : (1u << C::TS) - 1u);
+}
+
+// Asks for the rows of the tile from t0 in L2.
+template <class C>
+__device__ __forceinline__ void prefetch_tile(const PagedView& p, const PagedSeg& s, int t0) {
+  const int lane = threadIdx.x & 31, part = lane / C::TS;  // 32 / TS lanes a slot, 128 bytes at a time
+  const int t = t0 + (lane & (C::TS - 1));
+  if (t >= s.L) return;
+  int off;
+  const int page = slot_page(p, s.b, t, off);
+  if (page < 0) return;
+  const uint8_t* k = row_ptr(p.k, page, s.h, off);
+  const uint8_t* v = row_ptr(p.v, page, s.h, off);
+#pragma unroll
+  for (int o = 0; o < 2 * C::DP; o += 128 * (32 / C::TS)) {
+    const int x = o + 128 * part;
+    if (x < 2 * p.d) {
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(k + x));
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(v + x));
+    }
+  }
 }
 
 template <class C>
@@ -765,6 +794,12 @@ __global__ void __launch_bounds__(C::W * 32, C::MINB) k_paged_attn(const PagedVi
       at.valid = 0u;
       if (i + 1 < s.n) find_places<C>(p, a, s, tile_start(s, i + 1), at);
       else if (more) find_places<C>(p, a, ns, tile_start(ns, 0), at);
+      if constexpr (!C::Q) {
+        if (per > 16) {
+          if (i + 2 < s.n) prefetch_tile<C>(p, s, tile_start(s, i + 2));
+          else if (more && i + 2 - s.n < ns.n) prefetch_tile<C>(p, ns, tile_start(ns, i + 2 - s.n));
+        }
+      }
       float x[C::TT][C::NT][4];
       if (valid) tile_scores<C>(a, sm, f, x);
       if (at.valid) load_k<C>(p, at, f);
