@@ -53,13 +53,13 @@ class PagedKV:
     Only the last dimension has to be contiguous; row starts are 16-byte
     aligned.  A view: the tensors stay the caller's."""
 
-    __slots__ = ("k", "v", "scales", "device", "dtype", "shape", "head_dim", "bits", "_desc", "_index")
+    __slots__ = ("k", "v", "scales", "dtype", "shape", "head_dim", "bits", "_desc", "_index")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scales: torch.Tensor | None = None,
                  k_biases: torch.Tensor | None = None, v_scales: torch.Tensor | None = None,
                  v_biases: torch.Tensor | None = None):
-        kd, vd, dtype, dev = k.shape, v.shape, k.dtype, k.device
-        if len(kd) != 4 or len(vd) != 4 or kd[:3] != vd[:3] or dev.type != "cuda" or v.device != dev:
+        kd, vd, dtype, index = k.shape, v.shape, k.dtype, k.get_device()
+        if len(kd) != 4 or len(vd) != 4 or kd[:3] != vd[:3] or index < 0 or v.get_device() != index:
             raise ValueError("k and v must be CUDA tensors [pages, kv heads, page_size, ...] of the same pages")
         (k0, k1, k2, k3), (v0, v1, v2, v3) = k.stride(), v.stride()
         if k3 != 1 or v3 != 1:
@@ -79,7 +79,7 @@ class PagedKV:
             want = (*kd[:3], groups)
             a, b = k_scales.stride(), v_scales.stride()
             for t, st in ((k_scales, a), (k_biases, a), (v_scales, b), (v_biases, b)):
-                if t.dtype != _bf16 or t.shape != want or t.device != dev or t.stride() != st or st[3] != 1:
+                if t.dtype != _bf16 or t.shape != want or t.get_device() != index or t.stride() != st or st[3] != 1:
                     raise ValueError("scales and biases must be bf16 [pages, kv heads, page_size, head_dim / 64], "
                                      "those of one tensor with the same strides")
             if groups < 1 or kd[3] % (2 * groups) or vd[3] % (2 * groups):
@@ -90,8 +90,12 @@ class PagedKV:
                 k.data_ptr(), v.data_ptr(), k_scales.data_ptr(), k_biases.data_ptr(), v_scales.data_ptr(),
                 v_biases.data_ptr(), 4 * k0, 4 * k1, 4 * k2, 4 * v0, 4 * v1, 4 * v2, 2 * a[0], 2 * a[1], 2 * a[2],
                 2 * b[0], 2 * b[1], 2 * b[2], kd[0], kd[2], kd[1], 64 * groups, kb, vb, abi.REC_T_BF16)
-        self.k, self.v, self.device, self._index = k, v, dev, dev.index
+        self.k, self.v, self._index = k, v, index
         self.shape = kd[:3]
+
+    @property
+    def device(self) -> torch.device:
+        return self.k.device
 
     @classmethod
     def allocate(cls, pages: int, kv_heads: int, page_size: int, head_dim: int, *, k_bits: int = 16, v_bits: int = 16,
@@ -125,12 +129,13 @@ def _status_ptr(index: int) -> int | None:
     return s[1]
 
 
-def _buffers(call: str, device: torch.device, index: int, stream: int, need: int, zero: int) -> tuple:
+def _buffers(call: str, index: int, stream: int, need: int, zero: int) -> tuple:
     """(address, bytes, address, bytes) of the call's workspace and of its
     counters, which are zero between calls."""
     s = _scratch.get((call, index, stream))
     if s is not None and s[1][1] >= need and s[1][3] >= zero and not _capturing():
         return s[1]
+    device = torch.device("cuda", index)
     need, zero = max(need, 256), max(zero, 4096)
     if s is not None:
         need, zero = max(need, s[1][1]), max(zero, s[1][3])
@@ -157,22 +162,25 @@ def check_status(device=None) -> None:
         check(code)
 
 
-def _table(table: torch.Tensor, device: torch.device) -> tuple:
+def _table(table: torch.Tensor, index: int) -> tuple:
     """(the packed table, batch, width)."""
-    if table.dtype != _i32 or table.device != device or table.dim() != 2 or table.stride(1) != 1:
+    if table.dtype != _i32 or table.get_device() != index or table.dim() != 2:
         raise ValueError("the page table must be int32 [batch, pages] on the cache's device, rows contiguous")
     batch, width = table.shape
-    return _TABLE.pack(table.data_ptr(), table.stride(0), width, batch), batch, width
+    row, entry = table.stride()
+    if entry != 1 and width > 1:
+        raise ValueError("the page table's rows must be contiguous")
+    return _TABLE.pack(table.data_ptr(), row if batch > 1 else width, width, batch), batch, width
 
 
-def _ints(name: str, t: torch.Tensor, n: int, device: torch.device) -> int:
-    if t.dtype != _i32 or t.device != device or t.shape != (n,) or not t.is_contiguous():
+def _ints(name: str, t: torch.Tensor, n: int, index: int) -> int:
+    if t.dtype != _i32 or t.get_device() != index or t.shape != (n,) or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 tensor [{n}] on the cache's device")
     return t.data_ptr()
 
 
 def _per_slot(name: str, t: torch.Tensor, cache: PagedKV, dtype: torch.dtype) -> int:
-    if t.dtype != dtype or t.device != cache.device or t.shape != cache.shape or not t.is_contiguous():
+    if t.dtype != dtype or t.get_device() != cache._index or t.shape != cache.shape or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {dtype} tensor [pages, kv heads, page_size] on the cache's device")
     return t.data_ptr()
 
@@ -185,13 +193,13 @@ def paged_append(cache: PagedKV, k: torch.Tensor, v: torch.Tensor, table: torch.
     to slot starts[b] + r - cu_seqlens[b].  Quantized caches take the codes of
     rec_kv_append.  weights (fp32) and positions (int32), one value per slot:
     the written slots get 0 and their slot number."""
-    dev = cache.device
-    t, B, _ = _table(table, dev)
+    index = cache._index
+    t, B, _ = _table(table, index)
     heads, d, dtype = cache.shape[1], cache.head_dim, cache.dtype
     rows, want = k.shape[0], (k.shape[0], heads, d)
     (k0, k1, k2), (v0, v1, v2) = k.stride(), v.stride()
-    if k.dtype != dtype or v.dtype != dtype or k.shape != want or v.shape != want or k.device != dev \
-            or v.device != dev or k2 != 1 or v2 != 1 or (heads > 1 and (k1 != d or v1 != d)):
+    if k.dtype != dtype or v.dtype != dtype or k.shape != want or v.shape != want \
+            or k.get_device() != index or v.get_device() != index or k2 != 1 or v2 != 1 or (heads > 1 and (k1 != d or v1 != d)):
         raise ValueError(f"k and v must be {dtype} [rows, {heads}, {d}] on the cache's device, each row contiguous")
     if rows == 0:
         return
@@ -199,10 +207,10 @@ def paged_append(cache: PagedKV, k: torch.Tensor, v: torch.Tensor, table: torch.
         k0 = v0 = heads * d
     code = lib().rec_paged_append(
         cache._desc, t, k.data_ptr(), v.data_ptr(), k0, v0, rows,
-        _ints("cu_seqlens", cu_seqlens, B + 1, dev), _ints("starts", starts, B, dev),
+        _ints("cu_seqlens", cu_seqlens, B + 1, index), _ints("starts", starts, B, index),
         None if weights is None else _per_slot("weights", weights, cache, _f32),
         None if positions is None else _per_slot("positions", positions, cache, _i32),
-        _status_ptr(cache._index), _stream(cache._index))
+        _status_ptr(index), _stream(index))
     if code:
         check(code, "rec_paged_append")
 
@@ -223,24 +231,24 @@ def paged_attn_decode(cache: PagedKV, q: torch.Tensor, table: torch.Tensor, leng
     weights_out = decay * weights + the slot's softmax weights summed over the
     kv head's query heads, for every slot below the session's length;
     weights_out defaults to weights (in place)."""
-    dev, index, d = cache.device, cache._index, cache.head_dim
-    t, B, width = _table(table, dev)
+    index, d = cache._index, cache.head_dim
+    t, B, width = _table(table, index)
     shape = q.shape
-    if q.dtype != cache.dtype or len(shape) != 3 or shape[0] != B or shape[2] != d or q.device != dev \
+    if q.dtype != cache.dtype or len(shape) != 3 or shape[0] != B or shape[2] != d or q.get_device() != index \
             or q.stride(2) != 1:
         raise ValueError(f"q must be {cache.dtype} [{B}, query heads, {d}] on the cache's device, rows contiguous")
     if out is None:
-        out = torch.empty(shape, dtype=q.dtype, device=dev)
-    elif out.dtype != q.dtype or out.shape != shape or out.device != dev or out.stride(2) != 1:
+        out = q.new_empty(shape)
+    elif out.dtype != q.dtype or out.shape != shape or out.get_device() != index or out.stride(2) != 1:
         raise ValueError("out must match q, rows contiguous")
     hq = shape[1]
     lse_at = sinks_at = weights_at = weights_to = 0
     if lse is not None:
-        if lse.dtype != _f32 or lse.shape != (B, hq) or lse.device != dev or not lse.is_contiguous():
+        if lse.dtype != _f32 or lse.shape != (B, hq) or lse.get_device() != index or not lse.is_contiguous():
             raise ValueError(f"lse must be a contiguous fp32 tensor [{B}, {hq}] on the cache's device")
         lse_at = lse.data_ptr()
     if sinks is not None:
-        if sinks.dtype != _bf16 or sinks.shape != (hq,) or sinks.device != dev or not sinks.is_contiguous():
+        if sinks.dtype != _bf16 or sinks.shape != (hq,) or sinks.get_device() != index or not sinks.is_contiguous():
             raise ValueError(f"sinks must be a contiguous bf16 tensor [{hq}] on the cache's device")
         sinks_at = sinks.data_ptr()
     if weights is not None:
@@ -250,7 +258,7 @@ def paged_attn_decode(cache: PagedKV, q: torch.Tensor, table: torch.Tensor, leng
     if weights_out is not None:
         weights_to = _per_slot("weights_out", weights_out, cache, _f32)
     a = _ATTN.pack(q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1), lse_at,
-                   _ints("lengths", lengths, B, dev), sinks_at, hq, d ** -0.5 if scale is None else scale, softcap,
+                   _ints("lengths", lengths, B, index), sinks_at, hq, d ** -0.5 if scale is None else scale, softcap,
                    window, weights_at, weights_to, decay)
     L = lib()
     key = (index, B, width, hq, d, cache.shape, cache.bits, weights_to != 0)
@@ -262,7 +270,7 @@ def paged_attn_decode(cache: PagedKV, q: torch.Tensor, table: torch.Tensor, leng
         if need:
             _sizes[key] = size
     stream = _stream(index)
-    ws, ws_bytes, counters, counter_bytes = _buffers("attn", dev, index, stream, *size)
+    ws, ws_bytes, counters, counter_bytes = _buffers("attn", index, stream, *size)
     code = L.rec_paged_attn_decode(cache._desc, t, a, ws, ws_bytes, counters, counter_bytes, _status_ptr(index), stream)
     if code:
         check(code, "rec_paged_attn_decode")
@@ -287,10 +295,10 @@ def paged_evict(cache: PagedKV, table: torch.Tensor, lengths: torch.Tensor, budg
     counts as its own position.  weights_out and positions_out default to the
     inputs (in place).  The pages below the budget must not be shared with
     another session."""
-    dev, index = cache.device, cache._index
-    t, B, width = _table(table, dev)
+    index = cache._index
+    t, B, _ = _table(table, index)
     if lengths_out is None:
-        lengths_out = torch.empty(B, dtype=_i32, device=dev)
+        lengths_out = torch.empty_like(lengths)
     weights_at = weights_to = _per_slot("weights", weights, cache, _f32)
     positions_at = positions_to = keep_at = 0
     if weights_out is not None:
@@ -300,13 +308,13 @@ def paged_evict(cache: PagedKV, table: torch.Tensor, lengths: torch.Tensor, budg
     if positions_out is not None:
         positions_to = _per_slot("positions_out", positions_out, cache, _i32)
     if keep_from is not None:
-        keep_at = _ints("keep_from", keep_from, B, dev)
-    a = _EVICT.pack(_ints("lengths", lengths, B, dev), _ints("lengths_out", lengths_out, B, dev), budget, weights_at,
+        keep_at = _ints("keep_from", keep_from, B, index)
+    a = _EVICT.pack(_ints("lengths", lengths, B, index), _ints("lengths_out", lengths_out, B, index), budget, weights_at,
                     weights_to, positions_at, positions_to, keep_at, keep_below)
     L = lib()
     stream = _stream(index)
     need = L.rec_paged_evict_workspace_bytes(cache._desc, t, budget)
-    ws, ws_bytes, _, _ = _buffers("evict", dev, index, stream, need, 0)
+    ws, ws_bytes, _, _ = _buffers("evict", index, stream, need, 0)
     code = L.rec_paged_evict(cache._desc, t, a, ws, ws_bytes, _status_ptr(index), stream)
     if code:
         check(code, "rec_paged_evict")

@@ -194,11 +194,11 @@ _RULES = struct.Struct("@Pi4x7Pi4xPq")  # abi.RecLogitRules as one pack
 assert _RULES.size == C.sizeof(abi.RecLogitRules)
 
 
-def _per_row(name: str, x, batch: int, dtype: torch.dtype, device) -> torch.Tensor:
+def _per_row(name: str, x, batch: int, dtype: torch.dtype, index: int) -> torch.Tensor:
     """A contiguous [batch] tensor of `dtype`; a number is broadcast."""
     if not isinstance(x, torch.Tensor):
-        return torch.full((batch,), x, dtype=dtype, device=device)
-    if x.dtype != dtype or x.shape != (batch,) or x.device != device or not x.is_contiguous():
+        return torch.full((batch,), x, dtype=dtype, device=torch.device("cuda", index))
+    if x.dtype != dtype or x.shape != (batch,) or x.get_device() != index or not x.is_contiguous():
         raise ValueError(f"{name} must be a number or a contiguous {dtype} tensor [{batch}] on the logits' device")
     return x
 
@@ -221,50 +221,49 @@ def process_logits(logits: torch.Tensor, history: torch.Tensor | None = None,
     allow: 32-bit words [B, W], W >= ceil(V / 32), bit i & 31 of word i >> 5
     set for each allowed id; the others get -inf.  `out` may be `logits`.
     sample_logits with the penalties off samples from the result."""
-    kind, dev, shape = _LOGIT_TYPES.get(logits.dtype), logits.device, logits.shape
-    if kind is None or dev.type != "cuda" or len(shape) != 2 or logits.stride(1) != 1:
+    kind, index, shape = _LOGIT_TYPES.get(logits.dtype), logits.get_device(), logits.shape
+    if kind is None or index < 0 or len(shape) != 2 or logits.stride(1) != 1:
         raise ValueError("logits must be a bf16, fp16 or fp32 CUDA tensor [B, V] with contiguous rows")
     B, V = shape
-    index = dev.index
     if index != _current_device():
         raise ValueError("the tensors must live on the current CUDA device")
     if out is None:
-        out = torch.empty(shape, dtype=logits.dtype, device=dev)
-    elif out.dtype != logits.dtype or out.shape != shape or out.device != dev or out.stride(1) != 1:
+        out = logits.new_empty(shape)
+    elif out.dtype != logits.dtype or out.shape != shape or out.get_device() != index or out.stride(1) != 1:
         raise ValueError("out must match the logits, rows contiguous")
     if B == 0 or V == 0:
         return out
     hist = cap = len_at = prompt_at = ids_at = values_at = m = allow_at = allow_stride = 0
     rules = [None, None, None]  # kept until the launch
     if history is not None:
-        if history.dtype != torch.int32 or history.dim() != 2 or history.shape[0] != B or history.device != dev \
+        if history.dtype != torch.int32 or history.dim() != 2 or history.shape[0] != B or history.get_device() != index \
                 or not history.is_contiguous():
             raise ValueError("history must be a contiguous int32 tensor [B, n] on the logits' device")
         cap = history.shape[1]
         hist = history.data_ptr()
         if history_len is not None:
-            len_at = _per_row("history_len", history_len, B, torch.int32, dev).data_ptr()
+            len_at = _per_row("history_len", history_len, B, torch.int32, index).data_ptr()
         if prompt_len is not None:
-            prompt_at = _per_row("prompt_len", prompt_len, B, torch.int32, dev).data_ptr()
+            prompt_at = _per_row("prompt_len", prompt_len, B, torch.int32, index).data_ptr()
         if repetition is not None:
-            rules[0] = _per_row("repetition", repetition, B, torch.float32, dev)
+            rules[0] = _per_row("repetition", repetition, B, torch.float32, index)
         if frequency is not None:
-            rules[1] = _per_row("frequency", frequency, B, torch.float32, dev)
+            rules[1] = _per_row("frequency", frequency, B, torch.float32, index)
         if presence is not None:
-            rules[2] = _per_row("presence", presence, B, torch.float32, dev)
+            rules[2] = _per_row("presence", presence, B, torch.float32, index)
     elif history_len is not None or prompt_len is not None:
         raise ValueError("history_len and prompt_len need a history")
     if (bias_ids is None) != (bias_values is None):
         raise ValueError("bias_ids and bias_values come together")
     if bias_ids is not None:
         if bias_ids.dtype != torch.int32 or bias_values.dtype != torch.float32 or bias_ids.dim() != 2 \
-                or bias_ids.shape[0] != B or bias_values.shape != bias_ids.shape or bias_ids.device != dev \
-                or bias_values.device != dev or not bias_ids.is_contiguous() or not bias_values.is_contiguous():
+                or bias_ids.shape[0] != B or bias_values.shape != bias_ids.shape or bias_ids.get_device() != index \
+                or bias_values.get_device() != index or not bias_ids.is_contiguous() or not bias_values.is_contiguous():
             raise ValueError("bias_ids int32 and bias_values fp32 must be contiguous [B, m] on the logits' device")
         m = bias_ids.shape[1]
         ids_at, values_at = bias_ids.data_ptr(), bias_values.data_ptr()
     if allow is not None:
-        if allow.element_size() != 4 or allow.dim() != 2 or allow.shape[0] != B or allow.device != dev \
+        if allow.element_size() != 4 or allow.dim() != 2 or allow.shape[0] != B or allow.get_device() != index \
                 or allow.stride(1) != 1 or allow.shape[1] < (V + 31) // 32:
             raise ValueError("allow must be 32-bit words [B, >= ceil(V / 32)] on the logits' device, rows contiguous")
         allow_at, allow_stride = allow.data_ptr(), allow.stride(0)
