@@ -543,13 +543,14 @@ typedef struct RecPagedTable {
  * row r of session b, cu_dev[b] <= r < cu_dev[b + 1], goes to slot
  * starts_dev[b] + r - cu_dev[b] (K already RoPE'd).  Codes are formed as by
  * rec_kv_append.  weights (fp32) and positions (int32), both [n_pages]
- * [n_kv_heads][page_size] or NULL: the written slots get 0 and their slot
- * number.  A slot outside the table or a page outside the pool sets
+ * [n_kv_heads][page_size] or NULL: the written slots get 0 and their token's
+ * position, first_positions_dev[b] + r - cu_dev[b] (NULL: their slot number,
+ * which it is until the session's first eviction).  A slot outside the table or a page outside the pool sets
  * *status_dev and that row is not written. */
 REC_API int rec_paged_append(const RecPagedKV* kv, const RecPagedTable* table, const void* k_dev, const void* v_dev,
                              int64_t k_row_stride, int64_t v_row_stride, int64_t rows, const int32_t* cu_dev,
-                             const int32_t* starts_dev, float* weights, int32_t* positions, int32_t* status_dev,
-                             void* stream);
+                             const int32_t* starts_dev, float* weights, int32_t* positions,
+                             const int32_t* first_positions_dev, int32_t* status_dev, void* stream);
 
 /* Attention of one new token per session over its lengths[b] slots.
  *   s_t = scale * q . k_t, or softcap * tanh(s_t / softcap) for softcap > 0;
@@ -559,6 +560,8 @@ REC_API int rec_paged_append(const RecPagedKV* kv, const RecPagedTable* table, c
  * With weights_out, every slot t < L also gets
  *   weights_out[t] = decay * weights_in[t] + sum of p_t over the kv head's
  *   query heads   (weights_in may be weights_out; decay 0 reads nothing).
+ * The slots that take weights belong to one session each: sessions that share
+ * pages would overwrite one another's sums.
  * A page outside the pool sets *status_dev and its slots are left out. */
 typedef struct RecPagedAttn {
   const void* q;            /* [batch][n_q_heads][head_dim], 16-byte aligned */
@@ -632,7 +635,7 @@ typedef struct RecLogitRules {
   const float* bias_values;
   int32_t n_bias; /* < 8,191 */
   const uint32_t* allow;
-  int64_t allow_stride; /* words */
+  int64_t allow_stride; /* words, at least ceil(vocab / 32); 0: one mask for every row */
 } RecLogitRules;
 REC_API int rec_process_logits(const void* logits, int64_t stride, void* logits_out, int64_t out_stride, int32_t dtype,
                                int32_t batch, int32_t vocab, const RecLogitRules* rules, void* stream);

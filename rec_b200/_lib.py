@@ -83,7 +83,7 @@ _SIGNATURES = {
     "rec_set_layer_profile": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int32]),
     # structures of the batched calls: a ctypes reference or their packed bytes
     "rec_paged_append": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.c_int64,
-                                   C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
+                                   C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
     "rec_paged_attn_workspace_bytes": (C.c_size_t, [C.c_void_p, C.c_void_p, C.c_int32, C.c_int32,
                                                     C.POINTER(C.c_size_t)]),
     "rec_paged_attn_decode": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p,

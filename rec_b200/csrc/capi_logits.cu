@@ -194,7 +194,7 @@ REC_API int rec_process_logits(const void* logits, int64_t stride, void* logits_
                 "rec_process_logits: history of %d ids (at most %d)", r.history_cap, kMaxHistory);
   REC_CHECK_ARG(r.n_bias >= 0 && r.n_bias <= kMaxBias && (r.n_bias == 0 || (r.bias_ids && r.bias_values)),
                 "rec_process_logits: %d bias entries (at most %d)", r.n_bias, kMaxBias);
-  REC_CHECK_ARG(!r.allow || r.allow_stride >= (vocab + 31) / 32, "rec_process_logits: allow rows too short");
+  REC_CHECK_ARG(!r.allow || r.allow_stride == 0 || r.allow_stride >= (vocab + 31) / 32, "rec_process_logits: allow rows too short");
   LogitArgs a = {logits, logits_out, stride, out_stride, vocab, kMaxChunk, r};
   // whole waves of blocks, and at least 1,024 ids a block
   const int64_t wave = int64_t(sm_count()) * 4, span = int64_t(vocab) + 7;

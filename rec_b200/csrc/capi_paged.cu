@@ -100,6 +100,7 @@ struct AppendArgs {
   const int *cu, *starts;
   float* weights;
   int* positions;
+  const int* first;  // position of every session's first row, or NULL: its slot
   int* status;
 };
 
@@ -116,7 +117,7 @@ __device__ __forceinline__ int row_session(const int* cu, int batch, int64_t r) 
 // Where row r goes; page -1: nowhere (reported by the caller's first block of
 // threads that looks, `tell`).
 struct RowPlace {
-  int page, off, slot;
+  int page, off, position;
 };
 __device__ __forceinline__ RowPlace place_row(const PagedView& p, const AppendArgs& a, int64_t r, bool tell) {
   RowPlace w = {-1, 0, 0};
@@ -126,7 +127,7 @@ __device__ __forceinline__ RowPlace place_row(const PagedView& p, const AppendAr
   const int64_t slot = int64_t(__ldg(a.starts + b)) + (r - c0);
   const bool inside = slot >= 0 && slot < p.slots;
   if (inside) w.page = slot_page(p, b, int(slot), w.off);
-  w.slot = int(slot);
+  w.position = a.first ? int(__ldg(a.first + b) + (r - c0)) : int(slot);
   if (w.page < 0 && tell) report(a.status, inside ? kStatusBadPage : kStatusBadPosition);
   return w;
 }
@@ -135,7 +136,7 @@ __device__ __forceinline__ void mark_slots(const PagedView& p, const AppendArgs&
   if (w.page < 0) return;
   const int64_t at = slot_index(p, w.page, h, w.off);
   if (a.weights) a.weights[at] = 0.0f;
-  if (a.positions) a.positions[at] = w.slot;
+  if (a.positions) a.positions[at] = w.position;
 }
 
 constexpr int kAppendThreads = 256;
@@ -257,8 +258,8 @@ void launch_append(const PagedView& p, const AppendArgs& a, cudaStream_t st) {
 
 REC_API int rec_paged_append(const RecPagedKV* kv, const RecPagedTable* table, const void* k_dev, const void* v_dev,
                              int64_t k_row_stride, int64_t v_row_stride, int64_t rows, const int32_t* cu_dev,
-                             const int32_t* starts_dev, float* weights, int32_t* positions, int32_t* status_dev,
-                             void* stream) {
+                             const int32_t* starts_dev, float* weights, int32_t* positions,
+                             const int32_t* first_positions_dev, int32_t* status_dev, void* stream) {
   PagedView p;
   const int rc = paged_view(kv, table, "rec_paged_append", &p);
   if (rc) return rc;
@@ -271,7 +272,7 @@ REC_API int rec_paged_append(const RecPagedKV* kv, const RecPagedTable* table, c
   REC_CHECK_ARG(k_row_stride >= line && v_row_stride >= line && k_row_stride % 8 == 0 && v_row_stride % 8 == 0,
                 "rec_paged_append: row strides must be multiples of 8 elements and hold a row");
   AppendArgs a = {static_cast<const uint16_t*>(k_dev), static_cast<const uint16_t*>(v_dev), k_row_stride, v_row_stride,
-                  rows, cu_dev, starts_dev, weights, positions, status_dev};
+                  rows, cu_dev, starts_dev, weights, positions, first_positions_dev, status_dev};
   if (p.k_bits == 16) launch_append<false>(p, a, static_cast<cudaStream_t>(stream));
   else launch_append<true>(p, a, static_cast<cudaStream_t>(stream));
   REC_CHECK_CUDA(cudaGetLastError());

@@ -187,12 +187,14 @@ def _per_slot(name: str, t: torch.Tensor, cache: PagedKV, dtype: torch.dtype) ->
 
 def paged_append(cache: PagedKV, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, starts: torch.Tensor,
                  cu_seqlens: torch.Tensor, weights: torch.Tensor | None = None,
-                 positions: torch.Tensor | None = None) -> None:
+                 positions: torch.Tensor | None = None, first_positions: torch.Tensor | None = None) -> None:
     """Writes the new tokens' rows k, v [rows, kv heads, head_dim] (K already
     RoPE'd): row r of session b, cu_seqlens[b] <= r < cu_seqlens[b + 1], goes
     to slot starts[b] + r - cu_seqlens[b].  Quantized caches take the codes of
     rec_kv_append.  weights (fp32) and positions (int32), one value per slot:
-    the written slots get 0 and their slot number."""
+    the written slots get 0 and their token's position, first_positions[b]
+    (int32) + r - cu_seqlens[b]; without first_positions their slot number,
+    which it is until the session's first eviction."""
     index = cache._index
     t, B, _ = _table(table, index)
     heads, d, dtype = cache.shape[1], cache.head_dim, cache.dtype
@@ -210,9 +212,10 @@ def paged_append(cache: PagedKV, k: torch.Tensor, v: torch.Tensor, table: torch.
         _ints("cu_seqlens", cu_seqlens, B + 1, index), _ints("starts", starts, B, index),
         None if weights is None else _per_slot("weights", weights, cache, _f32),
         None if positions is None else _per_slot("positions", positions, cache, _i32),
+        None if first_positions is None else _ints("first_positions", first_positions, B, index),
         _status_ptr(index), _stream(index))
     if code:
-        check(code, "rec_paged_append")
+        check(code)
 
 
 def paged_attn_decode(cache: PagedKV, q: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, *,
@@ -230,7 +233,8 @@ def paged_attn_decode(cache: PagedKV, q: torch.Tensor, table: torch.Tensor, leng
     log) is filled when given.  weights (fp32, one value per slot) accumulate:
     weights_out = decay * weights + the slot's softmax weights summed over the
     kv head's query heads, for every slot below the session's length;
-    weights_out defaults to weights (in place)."""
+    weights_out defaults to weights (in place).  Slots that take weights belong
+    to one session each."""
     index, d = cache._index, cache.head_dim
     t, B, width = _table(table, index)
     shape = q.shape
@@ -273,7 +277,7 @@ def paged_attn_decode(cache: PagedKV, q: torch.Tensor, table: torch.Tensor, leng
     ws, ws_bytes, counters, counter_bytes = _buffers("attn", index, stream, *size)
     code = L.rec_paged_attn_decode(cache._desc, t, a, ws, ws_bytes, counters, counter_bytes, _status_ptr(index), stream)
     if code:
-        check(code, "rec_paged_attn_decode")
+        check(code)
     return out
 
 
@@ -317,5 +321,5 @@ def paged_evict(cache: PagedKV, table: torch.Tensor, lengths: torch.Tensor, budg
     ws, ws_bytes, _, _ = _buffers("evict", index, stream, need, 0)
     code = L.rec_paged_evict(cache._desc, t, a, ws, ws_bytes, _status_ptr(index), stream)
     if code:
-        check(code, "rec_paged_evict")
+        check(code)
     return lengths_out

@@ -219,7 +219,8 @@ def process_logits(logits: torch.Tensor, history: torch.Tensor | None = None,
     [B, m] (ids outside the vocabulary, such as -1, are ignored) with
     bias_values fp32 [B, m] are added, the last entry of an id counting.
     allow: 32-bit words [B, W], W >= ceil(V / 32), bit i & 31 of word i >> 5
-    set for each allowed id; the others get -inf.  `out` may be `logits`.
+    set for each allowed id; the others get -inf.  One mask may be expanded over
+    the rows.  `out` may be `logits`.
     sample_logits with the penalties off samples from the result."""
     kind, index, shape = _LOGIT_TYPES.get(logits.dtype), logits.get_device(), logits.shape
     if kind is None or index < 0 or len(shape) != 2 or logits.stride(1) != 1:
@@ -274,7 +275,7 @@ def process_logits(logits: torch.Tensor, history: torch.Tensor | None = None,
     s_in, s_out = (logits.stride(0), out.stride(0)) if B > 1 else (V, V)
     code = lib().rec_process_logits(logits.data_ptr(), s_in, out.data_ptr(), s_out, kind, B, V, r, _raw_stream(index))
     if code:
-        check(code, "rec_process_logits")
+        check(code)
     return out
 
 

@@ -55,7 +55,7 @@ def run_evict(k=None, t=None, ws=P, nbytes=1 << 30, **over):
 
 def run_append(k=None, t=None, kp=P, vp=P, ks=256, vs=256, rows=5, cu=P, starts=P):
     return _lib.lib().rec_paged_append(C.byref(k or kv()), C.byref(t or table()), kp, vp, ks, vs, rows, cu, starts, None,
-                                       None, None, None)
+                                       None, None, None, None)
 
 
 BAD_CACHES = [dict(k=0), dict(v=P + 8), dict(k_bits=8), dict(k_bits=3, v_bits=3), dict(k_bits=16, v_bits=8),
