@@ -103,6 +103,8 @@ REC_API int rec_paged_attn_decode(const RecPagedKV* kv, const RecPagedTable* tab
                 "rec_paged_attn_decode: bad scale, softcap or window");
   REC_CHECK_ARG(!t.weights_out || t.decay == 0.0f || t.weights_in,
                 "rec_paged_attn_decode: decay without weights_in");
+  // so that the units of all sessions (of 128 slots or more) fit 31 bits
+  REC_CHECK_ARG(p.batch * p.slots <= int64_t(1) << 37, "rec_paged_attn_decode: a table of %lld slots", (long long)(p.batch * p.slots));
   const Layout l = layout_of(p, t.n_q_heads, t.weights_out != nullptr);
   REC_CHECK_ARG(workspace && workspace_bytes >= l.total && (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0,
                 "rec_paged_attn_decode: workspace must be 256-byte aligned and hold %zu bytes", l.total);

@@ -7,7 +7,12 @@
 // neither a long session nor many short ones leave an SM idle.  A block walks
 // its share segment by segment (a segment: its units of one (session, head));
 // a segment that is not the whole list of its head leaves a partial state,
-// and the last block to finish a head joins the partials in block order.
+// and the last block to finish a head joins the partials in block order.  A
+// join takes about as long as two units (3.5 us), so where every head can have
+// a block of its own and none is longer than that beyond an even share, a
+// block takes a whole head (24 sessions, window 513: 14.6 -> 9.4 us; 300 slots
+// 9.5 -> 8.0; 500 slots 10.5 -> 10.1; 800 slots of 8-bit codes 11.2 -> 11.9;
+// three more units instead of two would make no difference).
 //
 // Tile.  A warp folds 16 * TT slots at a time on the tensor cores
 // (mma.m16n8k16), with the cache as the A operand so that 8 query heads fill
@@ -175,6 +180,7 @@ struct PagedSmem {
   float head_m[C::HN], head_l[C::HN];
   int scan[32];
   int last;
+  int64_t per;  // units of a block's share
   alignas(16) float acc[C::W][C::HN][C::RP];  // joins: weights of the partials
   // then: int len[batch], pre[batch + 1]
 };
@@ -743,11 +749,25 @@ __global__ void __launch_bounds__(C::W * 32, C::MINB) k_paged_attn(const PagedVi
   auto first_slot = [&](int L) { return a.window > 0 ? max(0, L - a.window) : 0; };
   plan_units(p, a.lengths, blockIdx.x == 0 ? a.status : nullptr, C::W * 32, len, pre, sm.scan,
              [&](int L) { return max(1, (L - first_slot(L) + C::UT - 1) / C::UT); });
-  const int64_t H = int64_t(p.hkv) * a.HB, total = pre[p.batch] * H;
-  const int64_t per = (total + gridDim.x - 1) / gridDim.x;
-  int64_t u = int64_t(blockIdx.x) * per;
-  const int64_t end = min(total, u + per);
-  if (u >= end) return;
+  const int64_t H = int64_t(p.hkv) * a.HB;
+  {
+    int64_t per = (pre[p.batch] * H + gridDim.x - 1) / gridDim.x;
+    if (int64_t(p.batch) * H <= gridDim.x) {
+      const int b = threadIdx.x, nb = b < p.batch ? pre[b + 1] - pre[b] : 0, most = int(per) + 2;
+      for (int k = int(per); k <= most; ++k)
+        if (!__syncthreads_or(nb > k)) {  // every head's units filled up to k: a block's share is a head
+          if (b <= p.batch) pre[b] = b * k;
+          per = k;
+          break;
+        }
+    }
+    if (threadIdx.x == 0) sm.per = per;  // (held there: the loop below has no registers to spare)
+    __syncthreads();
+  }
+  const int64_t total = pre[p.batch] * H;
+  int64_t u = int64_t(blockIdx.x) * sm.per;
+  auto end = [&] { return min(total, int64_t(blockIdx.x + 1) * sm.per); };
+  if (u >= end()) return;
 
   auto seg_at = [&](int b, int hh, int ul, int64_t at) {
     PagedSeg s;
@@ -758,7 +778,7 @@ __global__ void __launch_bounds__(C::W * 32, C::MINB) k_paged_attn(const PagedVi
     s.lo = first_slot(s.L);
     s.nb = pre[b + 1] - pre[b];
     s.ul = ul;
-    s.n = int(min(int64_t(s.nb - ul), end - at));
+    s.n = int(min(int64_t(s.nb - ul), end() - at));
     return s;
   };
   PagedSeg s;
@@ -780,7 +800,7 @@ __global__ void __launch_bounds__(C::W * 32, C::MINB) k_paged_attn(const PagedVi
   }
   while (true) {
     PagedSeg ns = s;
-    const bool more = u + s.n < end;
+    const bool more = u + s.n < end();
     if (more) {
       const bool wrap = s.hh + 1 == H;  // a block's units of one head are one segment
       ns = seg_at(wrap ? s.b + 1 : s.b, wrap ? 0 : s.hh + 1, 0, u + s.n);
@@ -795,7 +815,7 @@ __global__ void __launch_bounds__(C::W * 32, C::MINB) k_paged_attn(const PagedVi
       if (i + 1 < s.n) find_places<C>(p, a, s, tile_start(s, i + 1), at);
       else if (more) find_places<C>(p, a, ns, tile_start(ns, 0), at);
       if constexpr (!C::Q) {
-        if (per > 16) {
+        if (sm.per > 16) {
           if (i + 2 < s.n) prefetch_tile<C>(p, s, tile_start(s, i + 2));
           else if (more && i + 2 - s.n < ns.n) prefetch_tile<C>(p, ns, tile_start(ns, i + 2 - s.n));
         }
@@ -888,7 +908,7 @@ __global__ void __launch_bounds__(C::W * 32, C::MINB) k_paged_attn(const PagedVi
         if (a.lse2) a.lse2[s.b * a.hq + hq] = lse2;
       }
     };
-    const int slot = whole ? 0 : 2 * blockIdx.x + (int64_t(blockIdx.x) * per >= head0 ? 0 : 1);
+    const int slot = whole ? 0 : 2 * blockIdx.x + (int64_t(blockIdx.x) * sm.per >= head0 ? 0 : 1);
     for (int i = threadIdx.x; i < heads * (C::DP / 4); i += C::W * 32) {
       const int n = i / (C::DP / 4), d = 4 * (i % (C::DP / 4));
       float M = sm.m[0][n];
@@ -917,7 +937,7 @@ __global__ void __launch_bounds__(C::W * 32, C::MINB) k_paged_attn(const PagedVi
     if (!whole) {
       // the last of the head's blocks joins their partials, in block order
       __syncthreads();
-      const int c0 = int(head0 / per), c1 = int((head0 + s.nb - 1) / per), parts = c1 - c0 + 1;
+      const int c0 = int(head0 / sm.per), c1 = int((head0 + s.nb - 1) / sm.per), parts = c1 - c0 + 1;
       if (threadIdx.x == 0) {
         unsigned* c = a.counters + s.b * H + s.hh;
         __threadfence();  // after the barrier: every thread's partial comes before the count
@@ -929,7 +949,7 @@ __global__ void __launch_bounds__(C::W * 32, C::MINB) k_paged_attn(const PagedVi
       __syncthreads();
       if (sm.last) {
         float* wgt = &sm.acc[0][0][0];  // [HN][parts]
-        auto part_slot = [&](int c) { return 2 * c + (int64_t(c) * per >= head0 ? 0 : 1); };
+        auto part_slot = [&](int c) { return 2 * c + (int64_t(c) * sm.per >= head0 ? 0 : 1); };
         for (int n = warp; n < heads; n += C::W) {
           float M = -INFINITY;
           for (int c = lane; c < parts; c += 32) M = fmaxf(M, __ldcg(a.part_ml + int64_t(part_slot(c0 + c)) * C::HN + n).x);
