@@ -2,12 +2,14 @@
 //
 // Two kernels, both bound by latency and by the scattered rows' sectors.  The
 // first selects: a cluster of 1 to 8 blocks per (session, kv head) holds the
-// slots' rank keys in shared memory, finds the budget-th largest by three
-// radix passes (11, 11 and 10 bits; the blocks' histograms meet in distributed
-// shared memory), and lists the evicted slots below the budget and the kept
-// slots at or above it, each in slot order.  A block takes up to 8,192 slots
-// (8 a thread) before a second one joins it: a pass over a cluster costs about
-// 2 us, eight more keys a thread far less.  The second kernel moves the r-th
+// slots' rank keys in shared memory, finds the budget-th largest by up to
+// three radix passes (11, 11 and 10 bits; the blocks' histograms meet in
+// distributed shared memory; the passes end once every key that begins with
+// the bits found stays), and lists the evicted slots below the budget and the
+// kept slots at or above it, each in slot order.  32 rows of 4,352 slots take
+// 14 us, of them 2.5 for the lengths, the table and the weights one after
+// another, 4 for the three passes that weights with ties need; 32 rows of up
+// to 65,536 slots 29 us.  The second kernel moves the r-th
 // kept row to the r-th hole: lane m of a warp finds the places of move m and
 // moves its scales, weight and position, then the warp moves the rows in
 // 16-byte pieces, four on their way per lane.  Only holes are filled, so a cut
@@ -43,6 +45,7 @@ struct EvictArgs {
   int cap;
   uint32_t* keys;       // [rows][slots] when a block's keys exceed its shared memory, or NULL
   int cluster;
+  int four;             // weights and positions can be read four slots at a time
   int* status;
 };
 
@@ -50,7 +53,7 @@ struct SelectSmem {
   unsigned hist[3][kBins];  // read by the cluster's other blocks
   int scan[kWarps], scan2[kWarps];
   int pub[3];               // ties, holes, survivors of this block
-  int digit, want;
+  int digit[3], want[3], whole[3];
 };
 
 // Ascending in the rank order: 0 for NaN, ..., 0xFFFFFFFF protected.
@@ -61,16 +64,27 @@ __device__ __forceinline__ uint32_t rank_key(float w, bool keep) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);       // +inf: 0xFF800000
 }
 
-// One more in bin d for every lane that calls with on; together where the
+// One more in bin d[k] for every lane and k with on[k]; together where the
 // whole warp has one bin (weights that are all equal).
-__device__ __forceinline__ void count_digit(unsigned* hist, unsigned d, bool on) {
-  const unsigned in = __ballot_sync(0xffffffffu, on);
-  if (!in) return;
-  const unsigned d0 = __shfl_sync(0xffffffffu, d, __ffs(in) - 1);
-  if (__all_sync(0xffffffffu, !on || d == d0)) {
-    if ((threadIdx.x & 31) == 0) atomicAdd(&hist[d0], unsigned(__popc(in)));
-  } else if (on) {
-    atomicAdd(&hist[d], 1u);
+template <int N>
+__device__ __forceinline__ void count_digits(unsigned* hist, const unsigned (&d)[N], const bool (&on)[N]) {
+  unsigned lo = 0xFFFFFFFFu, hi = 0u, n = 0u;
+#pragma unroll
+  for (int k = 0; k < N; ++k)
+    if (on[k]) {
+      lo = min(lo, d[k]);
+      hi = max(hi, d[k]);
+      ++n;
+    }
+  lo = __reduce_min_sync(0xffffffffu, lo);
+  hi = __reduce_max_sync(0xffffffffu, hi);
+  if (lo == hi) {
+    n = __reduce_add_sync(0xffffffffu, n);
+    if ((threadIdx.x & 31) == 0) atomicAdd(&hist[lo], n);
+  } else {
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      if (on[k]) atomicAdd(&hist[d[k]], 1u);
   }
 }
 
@@ -85,6 +99,8 @@ __device__ __forceinline__ int warps_before(int v, int* scan, int& all) {
   return __reduce_add_sync(0xffffffffu, x);
 }
 
+// SHARED: the block's keys fit its shared memory.
+template <bool SHARED>
 __global__ void __launch_bounds__(kThreads) k_evict_select(const PagedView p, const EvictArgs a) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
   SelectSmem& sm = *reinterpret_cast<SelectSmem*>(smem_raw);
@@ -122,57 +138,100 @@ __global__ void __launch_bounds__(kThreads) k_evict_select(const PagedView p, co
   // this block's slots: [s0, s0 + n)
   const int slice = ((L + a.cluster - 1) / a.cluster + 31) & ~31;
   const int s0 = min(L, rank * slice), n = min(L, s0 + slice) - s0;
-  uint32_t* keys = a.keys ? a.keys + int64_t(row) * p.slots + s0
-                          : reinterpret_cast<uint32_t*>(smem_raw + sizeof(SelectSmem));
-  for (int i = threadIdx.x; i < 3 * kBins; i += kThreads) (&sm.hist[0][0])[i] = 0u;
-  __syncthreads();
+  uint32_t* keys = SHARED ? reinterpret_cast<uint32_t*>(smem_raw + sizeof(SelectSmem))
+                          : a.keys + int64_t(row) * p.slots + s0;
   const int from = a.keep_from ? a.keep_from[b] : INT_MAX;
-  constexpr int U = 8;  // slots of a thread on their way at once
-  for (int i0 = 0; i0 < n; i0 += U * kThreads) {
-    int64_t at[U];
-    float w[U];
-    int pos[U];
-#pragma unroll
-    for (int k = 0; k < U; ++k) {
-      const int i = i0 + k * kThreads + int(threadIdx.x);
-      at[k] = -1;
-      if (i >= n) continue;
+  // 8 slots of a thread on their way at once: two pieces of four, where a piece never crosses a page
+  // (32 rows of 65,536 slots: 63.5 us for the call with single loads, 55 with pieces)
+  auto slot_of = [&](int i0, int k) {
+    return i0 + (a.four ? 4 * ((k >> 2) * kThreads + int(threadIdx.x)) + (k & 3) : k * kThreads + int(threadIdx.x));
+  };
+  bool cleared = false;
+  for (int i0 = 0; i0 < n; i0 += 8 * kThreads) {
+    int64_t at[8];
+    float w[8];
+    int pos[8];
+    auto place = [&](int i) {
       int off;
       const int page = slot_page(p, b, s0 + i, off);
       if (page < 0) report(a.status, kStatusBadPage);
-      else at[k] = slot_index(p, page, h, off);
-    }
+      return page < 0 ? int64_t(-1) : slot_index(p, page, h, off);
+    };
+    if (a.four) {
 #pragma unroll
-    for (int k = 0; k < U; ++k) {
-      w[k] = at[k] >= 0 ? a.w_in[at[k]] : 0.0f;
-      pos[k] = at[k] >= 0 && a.p_in ? a.p_in[at[k]] : s0 + i0 + k * kThreads + int(threadIdx.x);
-    }
+      for (int k = 0; k < 8; k += 4) {
+        const int i = slot_of(i0, k);
+        at[k] = i < n ? place(i) : -1;
 #pragma unroll
-    for (int k = 0; k < U; ++k) {
-      const int i = i0 + k * kThreads + int(threadIdx.x);
-      if (i0 + k * kThreads >= n) break;  // for the whole block
+        for (int e = 1; e < 4; ++e) at[k + e] = at[k] < 0 ? -1 : at[k] + e;
+      }
+#pragma unroll
+      for (int k = 0; k < 8; k += 4) {
+        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        int4 y = make_int4(s0 + slot_of(i0, k), s0 + slot_of(i0, k + 1), s0 + slot_of(i0, k + 2), s0 + slot_of(i0, k + 3));
+        if (at[k] >= 0) {
+          x = *reinterpret_cast<const float4*>(a.w_in + at[k]);
+          if (a.p_in) y = *reinterpret_cast<const int4*>(a.p_in + at[k]);
+        }
+        w[k] = x.x, w[k + 1] = x.y, w[k + 2] = x.z, w[k + 3] = x.w;
+        pos[k] = y.x, pos[k + 1] = y.y, pos[k + 2] = y.z, pos[k + 3] = y.w;
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) at[k] = slot_of(i0, k) < n ? place(slot_of(i0, k)) : -1;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        w[k] = at[k] >= 0 ? a.w_in[at[k]] : 0.0f;
+        pos[k] = at[k] >= 0 && a.p_in ? a.p_in[at[k]] : s0 + slot_of(i0, k);
+      }
+    }
+    if (!cleared) {  // while the first loads are on their way
+      for (int i = threadIdx.x; i < 3 * kBins / 4; i += kThreads) reinterpret_cast<uint4*>(sm.hist)[i] = make_uint4(0u, 0u, 0u, 0u);
+      __syncthreads();
+      cleared = true;
+    }
+    unsigned d[8];
+    bool in[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int i = slot_of(i0, k);
       uint32_t key = 0u;  // also of a slot whose page is bad
-      if (at[k] >= 0) {
+      in[k] = i < n;
+      if (in[k] && at[k] >= 0) {
         key = rank_key(w[k], pos[k] >= from || pos[k] < a.keep_below);
         if (copies) copy_slot(at[k], s0 + i, w[k], pos[k]);
       }
-      if (i < n) keys[i] = key;
-      count_digit(sm.hist[0], key >> 21, i < n);
+      if (in[k]) keys[i] = key;
+      d[k] = key >> 21;
     }
+    count_digits(sm.hist[0], d, in);
   }
-  // the budget-th largest key T, and how many of its equals stay
+  if (n == 0) {  // a cluster's last blocks may have no slots
+    for (int i = threadIdx.x; i < 3 * kBins / 4; i += kThreads) reinterpret_cast<uint4*>(sm.hist)[i] = make_uint4(0u, 0u, 0u, 0u);
+    __syncthreads();
+  }
+  // the budget-th largest key's leading bits T, and how many of the keys that begin with them stay; once
+  // all of those do, the bits after them decide nothing (for weights that differ, mostly after 22 bits)
   uint32_t T = 0;
-  int want = budget;
+  int want = budget, shift = 21;
+  bool whole = false;
 #pragma unroll 1
   for (int pass = 0; pass < 3; ++pass) {
-    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+    shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
     const unsigned bins = pass == 2 ? 1024u : 2048u;
     if (pass > 0)
-      for (int i0 = 0; i0 < n; i0 += kThreads) {
-        const int i = i0 + threadIdx.x;
-        const uint32_t key = i < n ? keys[i] : 0u;
+      for (int i0 = 0; i0 < n; i0 += 4 * kThreads) {
+        unsigned d[4];
+        bool on[4];
         const int above = pass == 1 ? 21 : 10;
-        count_digit(sm.hist[pass], (key >> shift) & (bins - 1), i < n && (key >> above) == (T >> above));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int i = i0 + k * kThreads + int(threadIdx.x);
+          d[k] = i < n ? keys[i] : 0u;
+          on[k] = i < n && (d[k] >> above) == T;
+          d[k] = (d[k] >> shift) & (bins - 1);
+        }
+        if (__any_sync(0xffffffffu, on[0] || on[1] || on[2] || on[3])) count_digits(sm.hist[pass], d, on);
       }
     sync();
     // thread i sums bins 2(1023 - i) + 1 and 2(1023 - i): descending order
@@ -195,53 +254,69 @@ __global__ void __launch_bounds__(kThreads) k_evict_select(const PagedView p, co
     const int before = warps_before(__shfl_sync(0xffffffffu, x, 31), sm.scan, all) + x - c0 - c1;
     if (before < want && want <= before + c0 + c1) {
       const bool upper = want <= before + c1;
-      sm.digit = upper ? d + 1 : d;
-      sm.want = want - before - (upper ? 0 : c1);
+      const int rest = want - before - (upper ? 0 : c1);
+      sm.digit[pass] = upper ? d + 1 : d;
+      sm.want[pass] = rest;
+      sm.whole[pass] = rest == (upper ? c1 : c0);
     }
     __syncthreads();
-    T |= uint32_t(sm.digit) << shift;
-    want = sm.want;
-    __syncthreads();
+    T = (T << (pass == 2 ? 10 : 11)) | uint32_t(sm.digit[pass]);
+    want = sm.want[pass];
+    whole = sm.whole[pass];
+    if (whole) break;  // the same in every block
   }
-  // a warp's slots are contiguous, so ranks in slot order are prefix counts
-  const int chunk = ((n + kWarps - 1) / kWarps + 31) & ~31;
-  const int i_lo = min(n, warp * chunk), i_hi = min(n, i_lo + chunk);
-  int ties = 0;
-  for (int i0 = i_lo; i0 < i_hi; i0 += 32)
-    ties += __popc(__ballot_sync(0xffffffffu, i0 + lane < i_hi && keys[i0 + lane] == T));
-  int all;
-  int tie0 = warps_before(ties, sm.scan, all);
-  if (threadIdx.x == 0) sm.pub[0] = all;
-  sync();
+  // a thread's slots are contiguous, so ranks in slot order are prefix counts; an odd number of them, so
+  // that the threads' keys lie in different banks
+  const int span = ((n + kThreads - 1) / kThreads) | 1;
+  const int i_lo = min(n, int(threadIdx.x) * span), i_hi = min(n, i_lo + span);
+  auto lanes_before = [&](int v, int& sum) {
+    int x = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    sum = __shfl_sync(0xffffffffu, x, 31);
+    return x - v;
+  };
   // lane r of every warp reads block r's count
   auto of_peers = [&](int k, int& before) {
     const int x = lane < a.cluster ? *peer(&sm.pub[k], lane) : 0;
     before += __reduce_add_sync(0xffffffffu, lane < rank ? x : 0);
     return __reduce_add_sync(0xffffffffu, x);
   };
-  of_peers(0, tie0);
-  const unsigned below = (1u << lane) - 1u;
-  // keep / hole / survivor of the 32 slots from i0; tie counts on
-  auto classify = [&](int i0, int& tie, bool& keep, bool& hole, bool& high) {
-    const int i = i0 + lane, t = s0 + i;
-    const bool in = i < i_hi;
-    const uint32_t key = in ? keys[i] : 0u;
-    const unsigned eq = __ballot_sync(0xffffffffu, in && key == T);
-    keep = in && (key > T || (key == T && tie + __popc(eq & below) < want));
-    tie += __popc(eq);
-    hole = in && !keep && t < budget;
-    high = keep && t >= budget;
-  };
-  int holes = 0, highs = 0, tie = tie0;
-  for (int i0 = i_lo; i0 < i_hi; i0 += 32) {
-    bool keep, hole, high;
-    classify(i0, tie, keep, hole, high);
-    holes += __popc(__ballot_sync(0xffffffffu, hole));
-    highs += __popc(__ballot_sync(0xffffffffu, high));
+  int all, sum, tie0 = 0;
+  if (!whole) {
+    int ties = 0;
+    for (int i = i_lo; i < i_hi; ++i) ties += keys[i] == T;  // all 32 bits here
+    tie0 = lanes_before(ties, sum);
+    tie0 += warps_before(sum, sm.scan, all);
+    if (threadIdx.x == 0) sm.pub[0] = all;
+    sync();
+    of_peers(0, tie0);
+  } else {
+    want = INT_MAX;
   }
-  int hole_at = warps_before(holes, sm.scan, all);
+  auto each = [&](auto&& hole, auto&& high) {
+    int tie = tie0;
+    for (int i = i_lo; i < i_hi; ++i) {
+      const uint32_t key = keys[i] >> shift;
+      const bool keep = key > T || (key == T && tie++ < want);
+      const int t = s0 + i;
+      if (!keep && t < budget) hole(t);
+      if (keep && t >= budget) high(t);
+    }
+  };
+  int holes = 0, highs = 0;
+  each([&](int) { ++holes; }, [&](int) { ++highs; });
+  int high_at = lanes_before(highs, sum);
+  if (lane == 0) sm.scan2[warp] = sum;
+  int hole_at = lanes_before(holes, sum);
+  hole_at += warps_before(sum, sm.scan, all);  // its barrier is also that of scan2
   if (threadIdx.x == 0) sm.pub[1] = all;
-  int high_at = warps_before(highs, sm.scan2, all);
+  const int other = sm.scan2[lane];
+  high_at += __reduce_add_sync(0xffffffffu, lane < warp ? other : 0);
+  all = __reduce_add_sync(0xffffffffu, other);
   if (threadIdx.x == 0) sm.pub[2] = all;
   sync();
   const int moves = of_peers(1, hole_at);
@@ -249,16 +324,7 @@ __global__ void __launch_bounds__(kThreads) k_evict_select(const PagedView p, co
   if (rank == 0 && threadIdx.x == 0) a.counts[row] = moves;
   int* hole_list = a.holes + int64_t(row) * a.cap;
   int* high_list = a.highs + int64_t(row) * a.cap;
-  tie = tie0;
-  for (int i0 = i_lo; i0 < i_hi; i0 += 32) {
-    bool keep, hole, high;
-    classify(i0, tie, keep, hole, high);
-    const unsigned ho = __ballot_sync(0xffffffffu, hole), hi = __ballot_sync(0xffffffffu, high);
-    if (hole) hole_list[hole_at + __popc(ho & below)] = s0 + i0 + lane;
-    if (high) high_list[high_at + __popc(hi & below)] = s0 + i0 + lane;
-    hole_at += __popc(ho);
-    high_at += __popc(hi);
-  }
+  each([&](int t) { hole_list[hole_at++] = t; }, [&](int t) { high_list[high_at++] = t; });
   sync();  // a block's counts stay readable until every block has them
 }
 
@@ -353,12 +419,13 @@ EvictLayout evict_layout(int64_t slots, int batch, int hkv, int budget) {
   EvictLayout l;
   const int64_t rows = int64_t(batch) * hkv;
   auto slice = [&](int c) { return ((slots + c - 1) / c + 31) / 32 * 32; };
-  // more blocks per row while a block has more than 8,192 keys and every block has an SM (one block
+  // more blocks per row while a block has more than 4,096 keys and every block has an SM (one block
   // fills it: 8 sessions x 4 heads of 65,536 slots take 47 us in clusters of 4, 87 us in two waves of
-  // clusters of 8), or while the keys do not fit
+  // clusters of 8; of 4,352 slots 16.7 us in clusters of 2, 17.2 alone, 18.9 in clusters of 4), or while
+  // the keys do not fit
   l.cluster = 1;
   while (l.cluster < kMaxCluster && (slice(l.cluster) > kKeysInShared ||
-                                     (slice(l.cluster) > 8192 && rows * l.cluster * 2 <= sm_count())))
+                                     (slice(l.cluster) > 4096 && rows * l.cluster * 2 <= sm_count())))
     l.cluster *= 2;
   l.shared = slice(l.cluster) <= kKeysInShared;
   l.cap = int(slots < budget ? slots : budget);
@@ -411,6 +478,8 @@ REC_API int rec_paged_evict(const RecPagedKV* kv, const RecPagedTable* table, co
   a.cap = l.cap;
   a.keys = l.shared ? nullptr : reinterpret_cast<uint32_t*>(ws + l.keys);
   a.cluster = l.cluster;
+  // a piece of four consecutive slots never crosses a page, and is aligned
+  a.four = p.ps.d % 4 == 0 && aligned16(a.w_in) && (!a.p_in || aligned16(a.p_in));
   a.status = status_dev;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const size_t slice = size_t((p.slots + l.cluster - 1) / l.cluster + 31) / 32 * 32;
@@ -424,9 +493,13 @@ REC_API int rec_paged_evict(const RecPagedKV* kv, const RecPagedTable* table, co
   attr[0].val.clusterDim = {unsigned(l.cluster), 1, 1};
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  REC_CHECK_CUDA(set_smem_limit(reinterpret_cast<const void*>(&k_evict_select),
-                                sizeof(SelectSmem) + size_t(kKeysInShared) * 4));
-  REC_CHECK_CUDA(cudaLaunchKernelEx(&cfg, k_evict_select, p, a));
+  if (l.shared) {
+    REC_CHECK_CUDA(set_smem_limit(reinterpret_cast<const void*>(&k_evict_select<true>),
+                                  sizeof(SelectSmem) + size_t(kKeysInShared) * 4));
+    REC_CHECK_CUDA(cudaLaunchKernelEx(&cfg, k_evict_select<true>, p, a));
+  } else {
+    REC_CHECK_CUDA(cudaLaunchKernelEx(&cfg, k_evict_select<false>, p, a));
+  }
   const FastDiv per = make_fastdiv(unsigned(p.d * (p.k_bits + p.v_bits) / 128));
   // moves of a row: no more than the budget, nor than the slots above it.  32 a warp; 8 where that
   // leaves SMs idle
