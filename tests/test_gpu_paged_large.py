@@ -10,7 +10,7 @@ import numpy as np
 import pytest
 import torch
 
-from rec_b200 import paged
+from rec_b200 import paged, sampling
 from tests import paged_reference as ref
 
 pytestmark = pytest.mark.gpu
@@ -152,3 +152,28 @@ def test_append_many_rows(kind, bits, heads, d):
     want = torch.full_like(pos, -1)
     want[pg, :, off] = torch.from_numpy(slot.astype(np.int32)).cuda()[:, None].expand(-1, heads)
     assert torch.equal(pos, want) and torch.equal(w, torch.where(want >= 0, 0.0, 7.0))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("B,V,n,m", [(70, 100_003, 5000, 40), (700, 9_300, 300, 3), (40, 151_936, 9000, 2000)])
+def test_logit_rules_many_rows(dtype, B, V, n, m):
+    """A batch of more than one wave equals its rows one at a time, bit for bit
+    (those are held against the fp32 steps elsewhere)."""
+    g = torch.Generator(device="cuda").manual_seed(V)
+    i32 = dict(device="cuda", dtype=torch.int32)
+    x = (4 * torch.randn(B, V, device="cuda", generator=g)).to(dtype)
+    history = (torch.rand(B, n, device="cuda", generator=g) ** 3 * (V + 5)).int() - 2  # many repeats, some ids outside
+    used = torch.randint(0, n + 1, (B,), generator=g, **i32)
+    prompt = (used * torch.rand(B, device="cuda", generator=g)).int()
+    numbers = [lo + torch.rand(B, device="cuda", generator=g) for lo in (1.0, 0.0, 0.0)]
+    ids = (torch.rand(B, m, device="cuda", generator=g) ** 3 * V).int()
+    ids[:, ::7] = -1
+    ids[:, m // 2:] = history[:, :m - m // 2]
+    values = torch.randn(B, m, device="cuda", generator=g)
+    allow = torch.randint(-2 ** 31, 2 ** 31, (B, (V + 31) // 32), device="cuda", generator=g).int()
+    args = (history, used, prompt, *numbers, ids, values, allow)
+    got = sampling.process_logits(x, *args)
+    for b in range(0, B, 9):
+        want = sampling.process_logits(x[b:b + 1], *(t[b:b + 1] for t in args))
+        assert torch.equal(got[b], want[0])
+    assert torch.equal(sampling.process_logits(x, *args, out=x), got)
