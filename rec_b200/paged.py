@@ -58,40 +58,50 @@ class PagedKV:
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scales: torch.Tensor | None = None,
                  k_biases: torch.Tensor | None = None, v_scales: torch.Tensor | None = None,
                  v_biases: torch.Tensor | None = None):
-        kd, vd, dtype, index = k.shape, v.shape, k.dtype, k.get_device()
-        if len(kd) != 4 or len(vd) != 4 or kd[:3] != vd[:3] or index < 0 or v.get_device() != index:
-            raise ValueError("k and v must be CUDA tensors [pages, kv heads, page_size, ...] of the same pages")
-        (k0, k1, k2, k3), (v0, v1, v2, v3) = k.stride(), v.stride()
+        dtype, index = k.dtype, k.get_device()
+        if k.dim() != 4 or v.dim() != 4 or index < 0 or v.get_device() != index:
+            raise ValueError("k and v must be CUDA tensors [pages, kv heads, page_size, ...]")
+        pages, heads, page, kw = k.shape
+        pages_v, heads_v, page_v, vw = v.shape
+        if pages != pages_v or heads != heads_v or page != page_v:
+            raise ValueError("k and v must have the same pages")
+        k0, k1, k2, k3 = k.stride()
+        v0, v1, v2, v3 = v.stride()
         if k3 != 1 or v3 != 1:
             raise ValueError("the rows of k and v must be contiguous")
-        self.scales = scales = (k_scales, k_biases, v_scales, v_biases)
         kind = _TYPES.get(dtype)
         if kind is not None:
-            if v.dtype != dtype or kd != vd or scales != (None, None, None, None):
+            if v.dtype is not dtype or kw != vw \
+                    or not (k_scales is None and k_biases is None and v_scales is None and v_biases is None):
                 raise ValueError("16-bit pools: k and v of one type and shape, no scales")
-            self.head_dim, self.dtype, self.bits = kd[3], dtype, (16, 16)
+            self.head_dim, self.dtype, self.bits = kw, dtype, (16, 16)
             self._desc = _KV.pack(k.data_ptr(), v.data_ptr(), 0, 0, 0, 0, 2 * k0, 2 * k1, 2 * k2, 2 * v0, 2 * v1, 2 * v2,
-                                  0, 0, 0, 0, 0, 0, kd[0], kd[2], kd[1], kd[3], 16, 16, kind)
+                                  0, 0, 0, 0, 0, 0, pages, page, heads, kw, 16, 16, kind)
         else:
-            if k.element_size() != 4 or v.element_size() != 4 or any(t is None for t in scales):
+            if k.element_size() != 4 or v.element_size() != 4 or k_scales is None or k_biases is None \
+                    or v_scales is None or v_biases is None:
                 raise ValueError("pools must be bf16, fp16, or 32-bit code words with scales and biases")
-            groups = k_scales.shape[-1]
-            want = (*kd[:3], groups)
-            a, b = k_scales.stride(), v_scales.stride()
-            for t, st in ((k_scales, a), (k_biases, a), (v_scales, b), (v_biases, b)):
-                if t.dtype != _bf16 or t.shape != want or t.get_device() != index or t.stride() != st or st[3] != 1:
-                    raise ValueError("scales and biases must be bf16 [pages, kv heads, page_size, head_dim / 64], "
-                                     "those of one tensor with the same strides")
-            if groups < 1 or kd[3] % (2 * groups) or vd[3] % (2 * groups):
+            shape, a, b = k_scales.shape, k_scales.stride(), v_scales.stride()
+            if shape[:-1] != (pages, heads, page) or a[-1] != 1 or b[-1] != 1 \
+                    or k_biases.shape != shape or v_scales.shape != shape or v_biases.shape != shape \
+                    or k_biases.stride() != a or v_biases.stride() != b \
+                    or not (k_scales.dtype is k_biases.dtype is v_scales.dtype is v_biases.dtype is _bf16) \
+                    or not (k_scales.get_device() == k_biases.get_device() == v_scales.get_device()
+                            == v_biases.get_device() == index):
+                raise ValueError("scales and biases must be bf16 [pages, kv heads, page_size, head_dim / 64], "
+                                 "those of one tensor with the same strides")
+            groups = shape[3]
+            if groups < 1 or kw % (2 * groups) or vw % (2 * groups):
                 raise ValueError("code words do not match the scales' head_dim")
             self.head_dim, self.dtype = 64 * groups, _bf16
-            self.bits = kb, vb = kd[3] // (2 * groups), vd[3] // (2 * groups)
+            self.bits = kb, vb = kw // (2 * groups), vw // (2 * groups)
             self._desc = _KV.pack(
                 k.data_ptr(), v.data_ptr(), k_scales.data_ptr(), k_biases.data_ptr(), v_scales.data_ptr(),
                 v_biases.data_ptr(), 4 * k0, 4 * k1, 4 * k2, 4 * v0, 4 * v1, 4 * v2, 2 * a[0], 2 * a[1], 2 * a[2],
-                2 * b[0], 2 * b[1], 2 * b[2], kd[0], kd[2], kd[1], 64 * groups, kb, vb, abi.REC_T_BF16)
+                2 * b[0], 2 * b[1], 2 * b[2], pages, page, heads, 64 * groups, kb, vb, abi.REC_T_BF16)
         self.k, self.v, self._index = k, v, index
-        self.shape = kd[:3]
+        self.scales = (k_scales, k_biases, v_scales, v_biases)
+        self.shape = (pages, heads, page)
 
     @property
     def device(self) -> torch.device:
@@ -174,7 +184,7 @@ def _table(table: torch.Tensor, index: int) -> tuple:
 
 
 def _ints(name: str, t: torch.Tensor, n: int, index: int) -> int:
-    if t.dtype != _i32 or t.get_device() != index or t.shape != (n,) or not t.is_contiguous():
+    if t.dtype is not _i32 or t.get_device() != index or t.shape != (n,) or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 tensor [{n}] on the cache's device")
     return t.data_ptr()
 
@@ -242,7 +252,7 @@ def paged_attn_decode(cache: PagedKV, q: torch.Tensor, table: torch.Tensor, leng
             or q.stride(2) != 1:
         raise ValueError(f"q must be {cache.dtype} [{B}, query heads, {d}] on the cache's device, rows contiguous")
     if out is None:
-        out = q.new_empty(shape)
+        out = torch.empty_like(q)
     elif out.dtype != q.dtype or out.shape != shape or out.get_device() != index or out.stride(2) != 1:
         raise ValueError("out must match q, rows contiguous")
     hq = shape[1]

@@ -229,7 +229,7 @@ def process_logits(logits: torch.Tensor, history: torch.Tensor | None = None,
     if index != _current_device():
         raise ValueError("the tensors must live on the current CUDA device")
     if out is None:
-        out = logits.new_empty(shape)
+        out = torch.empty_like(logits)
     elif out.dtype != logits.dtype or out.shape != shape or out.get_device() != index or out.stride(1) != 1:
         raise ValueError("out must match the logits, rows contiguous")
     if B == 0 or V == 0:
