@@ -26,7 +26,7 @@ __global__ void __launch_bounds__(kWeightThreads) k_paged_weights(const PagedVie
   int* pre = plan + p.batch;
   plan_units(p, a.lengths, nullptr, kWeightThreads, len, pre, scan,
              [](int L) { return max(1, (L + kWeightThreads - 1) / kWeightThreads); });
-  grid_wait();  // launched while the attention ends
+  grid_wait();  // launched while the attention ends; what it wrote is read by plain loads, which stay below
   const int64_t H = p.hkv, total = pre[p.batch] * H;
   for (int64_t u = blockIdx.x; u < total; u += gridDim.x) {
     const int b = unit_session(pre, p.batch, H, u);
@@ -44,11 +44,11 @@ __global__ void __launch_bounds__(kWeightThreads) k_paged_weights(const PagedVie
       // the scores of a slot's heads lie together; four at a time where a row of them is aligned
       if (a.G % 4 == 0) {
         for (int g = 0; g < a.G; g += 4) {
-          const float4 x = __ldcs(reinterpret_cast<const float4*>(sc + g));
+          const float4 x = *reinterpret_cast<const float4*>(sc + g);
           w += ex2(x.x - ls[g]) + ex2(x.y - ls[g + 1]) + ex2(x.z - ls[g + 2]) + ex2(x.w - ls[g + 3]);
         }
       } else {
-        for (int g = 0; g < a.G; ++g) w += ex2(__ldcs(sc + g) - ls[g]);
+        for (int g = 0; g < a.G; ++g) w += ex2(sc[g] - ls[g]);
       }
     }
     const int64_t at = slot_index(p, page, h, off);

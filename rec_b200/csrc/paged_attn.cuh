@@ -940,9 +940,9 @@ __global__ void __launch_bounds__(C::W * 32, C::MINB) k_paged_attn(const PagedVi
       const int c0 = int(head0 / sm.per), c1 = int((head0 + s.nb - 1) / sm.per), parts = c1 - c0 + 1;
       if (threadIdx.x == 0) {
         unsigned* c = a.counters + s.b * H + s.hh;
-        __threadfence();  // after the barrier: every thread's partial comes before the count
-        const unsigned before = atomicAdd(c, 1u);
-        __threadfence();
+        // releases the block's partials (the barrier above orders them before), acquires the others'
+        unsigned before;
+        asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(before) : "l"(c) : "memory");
         sm.last = before == unsigned(parts - 1);
         if (sm.last) *c = 0u;
       }
