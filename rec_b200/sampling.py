@@ -215,7 +215,8 @@ def process_logits(logits: torch.Tensor, history: torch.Tensor | None = None,
     history int32 [B, n] with history_len int32 [B] ids in use (default n):
     ids in it take `repetition` (x < 0 ? x * r : x / r); the c occurrences
     from prompt_len (int32 [B], default 0) on take `frequency` * c and, once,
-    `presence`.  Each of the three is a number or fp32 [B].  bias_ids int32
+    `presence`.  Each of the three is a number or fp32 [B], and the two lengths
+    may be one number for every row.  bias_ids int32
     [B, m] (ids outside the vocabulary, such as -1, are ignored) with
     bias_values fp32 [B, m] are added, the last entry of an id counting.
     allow: 32-bit words [B, W], W >= ceil(V / 32), bit i & 31 of word i >> 5
@@ -235,7 +236,7 @@ def process_logits(logits: torch.Tensor, history: torch.Tensor | None = None,
     if B == 0 or V == 0:
         return out
     hist = cap = len_at = prompt_at = ids_at = values_at = m = allow_at = allow_stride = 0
-    rules = [None, None, None]  # kept until the launch
+    rules = [None] * 5  # held until the launch: a number's tensor is made here
     if history is not None:
         if history.dtype != torch.int32 or history.dim() != 2 or history.shape[0] != B or history.get_device() != index \
                 or not history.is_contiguous():
@@ -243,9 +244,11 @@ def process_logits(logits: torch.Tensor, history: torch.Tensor | None = None,
         cap = history.shape[1]
         hist = history.data_ptr()
         if history_len is not None:
-            len_at = _per_row("history_len", history_len, B, torch.int32, index).data_ptr()
+            rules[3] = _per_row("history_len", history_len, B, torch.int32, index)
+            len_at = rules[3].data_ptr()
         if prompt_len is not None:
-            prompt_at = _per_row("prompt_len", prompt_len, B, torch.int32, index).data_ptr()
+            rules[4] = _per_row("prompt_len", prompt_len, B, torch.int32, index)
+            prompt_at = rules[4].data_ptr()
         if repetition is not None:
             rules[0] = _per_row("repetition", repetition, B, torch.float32, index)
         if frequency is not None:
@@ -270,7 +273,7 @@ def process_logits(logits: torch.Tensor, history: torch.Tensor | None = None,
         allow_at, allow_stride = allow.data_ptr(), allow.stride(0)
         if B == 1:
             allow_stride = allow.shape[1]  # a single row's stride is never used
-    rep, freq, pres = (0 if x is None else x.data_ptr() for x in rules)
+    rep, freq, pres = (0 if x is None else x.data_ptr() for x in rules[:3])
     r = _RULES.pack(hist, cap, len_at, prompt_at, rep, freq, pres, ids_at, values_at, m, allow_at, allow_stride)
     s_in, s_out = (logits.stride(0), out.stride(0)) if B > 1 else (V, V)
     code = lib().rec_process_logits(logits.data_ptr(), s_in, out.data_ptr(), s_out, kind, B, V, r, _raw_stream(index))
