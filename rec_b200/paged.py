@@ -10,12 +10,14 @@ the pool or a slot outside the table is left out and recorded on the device:
 
 Scratch memory is kept per (device, stream) and grows with the largest call,
 so calls on different streams do not meet; a call under stream capture takes
-its scratch from the capture's own pool.
+its scratch from the capture's own pool.  Threads may share a stream: a lock
+keeps one call's launches together.
 """
 from __future__ import annotations
 
 import ctypes as C
 import struct
+import threading
 
 import torch
 
@@ -26,6 +28,11 @@ from .ops import current_device as _current_device, raw_stream as _raw_stream
 _TYPES = {torch.bfloat16: abi.REC_T_BF16, torch.float16: abi.REC_T_FP16}
 _status: dict[int, tuple] = {}  # device -> (one word, its address)
 _scratch: dict[tuple, tuple] = {}  # (call, device, stream) -> (tensors, addresses and sizes)
+# Held from the lookup of a call's scratch to its last launch: the library is
+# called without the interpreter's lock, and another thread's call on the same
+# stream would replace the scratch before this one's launch, or launch between
+# this one's two kernels.
+_lock = threading.Lock()
 _sizes: dict[tuple, tuple] = {}  # shape of a call -> scratch bytes
 
 # The C structures of abi.py as one pack each: a step makes these calls once
@@ -135,26 +142,27 @@ def _status_ptr(index: int) -> int | None:
             return None  # cleared by every replay if it were captured
         t = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", index))
         torch.cuda.current_stream(index).synchronize()  # zero before any other stream's call
-        s = _status[index] = (t, t.data_ptr())
+        s = _status.setdefault(index, (t, t.data_ptr()))  # the first thread's word
     return s[1]
 
 
 def _buffers(call: str, index: int, stream: int, need: int, zero: int) -> tuple:
-    """(address, bytes, address, bytes) of the call's workspace and of its
-    counters, which are zero between calls."""
+    """The call's workspace and its counters, which are zero between calls:
+    the tensors, which the caller holds until the launch, and (address, bytes,
+    address, bytes).  Called with the lock held."""
     s = _scratch.get((call, index, stream))
     if s is not None and s[1][1] >= need and s[1][3] >= zero and not _capturing():
-        return s[1]
+        return s
     device = torch.device("cuda", index)
     need, zero = max(need, 256), max(zero, 4096)
     if s is not None:
         need, zero = max(need, s[1][1]), max(zero, s[1][3])
     ws = torch.empty(need, dtype=torch.uint8, device=device)
     counters = torch.zeros(zero, dtype=torch.uint8, device=device)
-    at = (ws.data_ptr(), need, counters.data_ptr(), zero)
+    s = ((ws, counters), (ws.data_ptr(), need, counters.data_ptr(), zero))
     if not _capturing():
-        _scratch[(call, index, stream)] = ((ws, counters), at)
-    return at
+        _scratch[(call, index, stream)] = s
+    return s
 
 
 def check_status(device=None) -> None:
@@ -284,8 +292,9 @@ def paged_attn_decode(cache: PagedKV, q: torch.Tensor, table: torch.Tensor, leng
         if need:
             _sizes[key] = size
     stream = _stream(index)
-    ws, ws_bytes, counters, counter_bytes = _buffers("attn", index, stream, *size)
-    code = L.rec_paged_attn_decode(cache._desc, t, a, ws, ws_bytes, counters, counter_bytes, _status_ptr(index), stream)
+    with _lock:
+        held, at = _buffers("attn", index, stream, *size)
+        code = L.rec_paged_attn_decode(cache._desc, t, a, *at, _status_ptr(index), stream)
     if code:
         check(code)
     return out
@@ -328,8 +337,9 @@ def paged_evict(cache: PagedKV, table: torch.Tensor, lengths: torch.Tensor, budg
     L = lib()
     stream = _stream(index)
     need = L.rec_paged_evict_workspace_bytes(cache._desc, t, budget)
-    ws, ws_bytes, _, _ = _buffers("evict", index, stream, need, 0)
-    code = L.rec_paged_evict(cache._desc, t, a, ws, ws_bytes, _status_ptr(index), stream)
+    with _lock:
+        held, at = _buffers("evict", index, stream, need, 0)
+        code = L.rec_paged_evict(cache._desc, t, a, at[0], at[1], _status_ptr(index), stream)
     if code:
         check(code)
     return lengths_out
