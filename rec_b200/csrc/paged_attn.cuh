@@ -31,12 +31,15 @@
 // Loads on their way hold L1 space, so shared memory is kept small: 227 KB of
 // it instead of 54 took the same case from 188 to 241 us.
 //
-// Softmax.  s in log2 units; m is a reference per head that follows the
-// running maximum when it is passed by more than 8 (p <= 256 until then), so
+// Softmax.  s in log2 units; a reference per head follows the running maximum
+// when it is passed by more than 8 (bf16: p <= 256 until then) or 4 (fp16), so
 // most tiles need no reduction over the warp and no rescaling.  p enters the
-// PV product as two 16-bit numbers, high and low part (a relative 2^-16 for
-// bf16), so the output keeps fp32 quality before its one rounding; the second
-// MMA is free, the kernel is bound by the cache's bytes.
+// PV product as two 16-bit numbers, high and low part: a relative 2^-16 for
+// bf16.  fp16 ends at 2^-24, so there the reference lies 2^9 below the maximum:
+// two parts keep 2^-22 of p, and no less than 2^-34 of the largest weight in
+// the warp, where p against the maximum itself would lose every weight below
+// 2^-25 of it whole.  The second MMA is free, the kernel is bound by the
+// cache's bytes (64 sessions up to 8K of fp16: 105 us with either reference).
 //
 // Quantized rows.  score = sum_g scale_g (q . c_g) + bias_g sum(q_g) over the
 // 64-dim groups, with the codes centred (c - 128 or c - 8: exact in fp16, and
@@ -169,6 +172,9 @@ struct PagedCfg {
   static constexpr int SW = (NG + 1) / 2;                                // words of a row's scales
   static constexpr int QP = DP + 32;                                     // pitch of a query in shared memory
   static constexpr int RP = DP + 4;                                      // pitch of a head's state there
+  // The reference moves when a score passes the maximum by more than LAG, and then lies REF below it: fp16
+  // rows take p from 2^9 (at the maximum) up to 2^14, bf16 needs no such place.
+  static constexpr float LAG = F16 && !Q ? 4.0f : 8.0f, REF = F16 && !Q ? 9.0f : 0.0f;
 };
 
 template <class C>
@@ -540,7 +546,7 @@ __device__ __forceinline__ void tile_fold(PagedTile<C>& f, uint32_t valid, float
       }
     }
   }
-  // the reference follows the maximum when it is passed by more than 8
+  // the reference follows the maximum when it is passed by more than LAG
   float top[C::NT][2];
   bool move = false;
 #pragma unroll
@@ -551,7 +557,7 @@ __device__ __forceinline__ void tile_fold(PagedTile<C>& f, uint32_t valid, float
 #pragma unroll
       for (int mt = 1; mt < C::TT; ++mt) t = fmaxf(t, fmaxf(x[mt][nt][e], x[mt][nt][2 + e]));
       top[nt][e] = t;
-      move |= t > st.m[nt][e] + 8.0f;
+      move |= t > st.m[nt][e] + C::LAG;
     }
   float big = 0.0f;  // codes: the largest |scale|, in acc's units
   if constexpr (C::Q) {
@@ -579,8 +585,8 @@ __device__ __forceinline__ void tile_fold(PagedTile<C>& f, uint32_t valid, float
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
         const float mn = fmaxf(st.m[nt][e], t);
-        const float mu = mn == -INFINITY ? 0.0f : mn;
-        const float al = ex2(st.m[nt][e] - mu);  // 0 while the old maximum is -inf (the state is 0 then)
+        const float mu = mn == -INFINITY ? 0.0f : mn - C::REF;
+        const float al = st.m[nt][e] == -INFINITY ? 0.0f : ex2(st.mu[nt][e] - mu);  // (the state is 0 then)
         st.m[nt][e] = mn;
         st.mu[nt][e] = mu;
         st.l[nt][e] *= al;
@@ -863,7 +869,7 @@ __global__ void __launch_bounds__(C::W * 32, C::MINB) k_paged_attn(const PagedVi
           }
         }
         if (j == 0) {
-          sm.m[warp][n] = st.m[nt][e];
+          sm.m[warp][n] = st.m[nt][e] == -INFINITY ? -INFINITY : st.mu[nt][e];
           sm.l[warp][n] = l;
         }
         const float back = C::Q ? (st.vf == 0.0f ? 1.0f : 1.0f / st.vf) : 1.0f;
