@@ -45,11 +45,15 @@
 // 64-dim groups, with the codes centred (c - 128 or c - 8: exact in fp16, and
 // the bias term then cancels little); q enters as fp16 after a power of two
 // that brings the head's largest value into [1, 2), so what fp16 loses is
-// below 2^-25 of it.  PV: p * scale_g is the P operand of group g (times a
-// power of two that follows the largest scale seen), rounded to fp16: a
-// relative 2^-12 per slot, a tenth of the output's own bf16 rounding, so its
-// low part is left out.  sum p * bias_g is added to the group's dims at the
-// end, in fp32.
+// below 2^-25 of it.  PV: p * scale_g is the P operand of group g, in two fp16
+// parts as above.  Its size is what has to fit fp16, so the reference follows
+// the maximum of score + log2(largest |scale| of the slot): p itself is fp32
+// and takes any unit, and a slot whose scale is large but whose weight is
+// small costs the others nothing.  The warps' units meet again when a segment
+// ends (each state brought to a sum in [1, 2)).  sum p * bias_g is added to the
+// group's dims there, in fp32.  One fp16 part (2^-11 of a weight) would be 4 to
+// 5 % faster (131,072 slots of 8 bits 42.9 against 44.9 us) and would move
+// outputs by 7.5e-4 in the 2-norm.
 #pragma once
 #include "paged.cuh"
 
@@ -173,8 +177,9 @@ struct PagedCfg {
   static constexpr int QP = DP + 32;                                     // pitch of a query in shared memory
   static constexpr int RP = DP + 4;                                      // pitch of a head's state there
   // The reference moves when a score passes the maximum by more than LAG, and then lies REF below it: fp16
-  // rows take p from 2^9 (at the maximum) up to 2^14, bf16 needs no such place.
-  static constexpr float LAG = F16 && !Q ? 4.0f : 8.0f, REF = F16 && !Q ? 9.0f : 0.0f;
+  // MMAs take p from 2^9 (at the maximum) up to 2^14 (codes: p * scale, below 2^15), bf16 needs no such place.
+  // (LAG 2 and REF 11 would gain two bits and cost codes 0.5 %.)
+  static constexpr float LAG = F16 ? 4.0f : 8.0f, REF = F16 ? 9.0f : 0.0f;
 };
 
 template <class C>
@@ -387,7 +392,6 @@ struct PagedState {
   float m[C::NT][2], mu[C::NT][2], l[C::NT][2];  // maximum, the reference in use (0 while m is -inf), lane's part of the sum
   float acc[C::NT][C::NG][4][4];
   float xb[C::NT][2][C::Q ? C::NG : 1];          // codes: sum of p * bias
-  float vf;                                      // codes: acc is in units of 1 / vf
   __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int nt = 0; nt < C::NT; ++nt) {
@@ -405,7 +409,6 @@ struct PagedState {
 #pragma unroll
           for (int c = 0; c < 4; ++c) acc[nt][g][i][c] = 0.0f;
     }
-    vf = 0.0f;
   }
 };
 
@@ -547,36 +550,33 @@ __device__ __forceinline__ void tile_fold(PagedTile<C>& f, uint32_t valid, float
     }
   }
   // the reference follows the maximum when it is passed by more than LAG
+  float es[C::TT][2];  // codes: log2 of the largest |scale| of rows j, j + 8, below by less than 1
+  if constexpr (C::Q) {
+    float big = 0.0f;
+#pragma unroll
+    for (int g = 0; g < C::NG; ++g) big = fmaxf(big, fabsf(scale_of(f.vs, g)));
+    // (rec_kv_append's scales are 2^-24 or more; the bounds keep two references' distance inside ex2's range)
+    const float own = float(min(96, max(-24, int(__float_as_uint(big) >> 23) - 127)));
+#pragma unroll
+    for (int mt = 0; mt < C::TT; ++mt)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) es[mt][r] = __shfl_sync(0xffffffffu, own, 16 * mt + 8 * r + j);
+  }
   float top[C::NT][2];
   bool move = false;
 #pragma unroll
   for (int nt = 0; nt < C::NT; ++nt)
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      float t = fmaxf(x[0][nt][e], x[0][nt][2 + e]);
+      float t = -INFINITY;
 #pragma unroll
-      for (int mt = 1; mt < C::TT; ++mt) t = fmaxf(t, fmaxf(x[mt][nt][e], x[mt][nt][2 + e]));
+      for (int mt = 0; mt < C::TT; ++mt)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) t = fmaxf(t, C::Q ? x[mt][nt][2 * r + e] + es[mt][r] : x[mt][nt][2 * r + e]);
       top[nt][e] = t;
       move |= t > st.m[nt][e] + C::LAG;
     }
-  float big = 0.0f;  // codes: the largest |scale|, in acc's units
-  if constexpr (C::Q) {
-#pragma unroll
-    for (int g = 0; g < C::NG; ++g) big = fmaxf(big, fabsf(scale_of(f.vs, g)));
-    move |= st.vf == 0.0f || big * st.vf > 64.0f;
-  }
   if (__any_sync(0xffffffffu, move)) {
-    float unit = 1.0f;
-    if constexpr (C::Q) {
-      big = bfly_max(big);
-      if (st.vf == 0.0f || big * st.vf > 64.0f) {
-        // the power of two that brings the largest scale into [16, 32)
-        const int e = min(230, max(20, int(__float_as_uint(big) >> 23)));
-        const float vf = __int_as_float((258 - e) << 23);
-        unit = st.vf == 0.0f ? 1.0f : vf / st.vf;
-        st.vf = vf;
-      }
-    }
 #pragma unroll
     for (int nt = 0; nt < C::NT; ++nt)
 #pragma unroll
@@ -585,7 +585,8 @@ __device__ __forceinline__ void tile_fold(PagedTile<C>& f, uint32_t valid, float
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
         const float mn = fmaxf(st.m[nt][e], t);
-        const float mu = mn == -INFINITY ? 0.0f : mn - C::REF;
+        // codes: whole, so that states are brought to another reference by powers of two
+        const float mu = mn == -INFINITY ? 0.0f : (C::Q ? floorf(mn) : mn) - C::REF;
         const float al = st.m[nt][e] == -INFINITY ? 0.0f : ex2(st.mu[nt][e] - mu);  // (the state is 0 then)
         st.m[nt][e] = mn;
         st.mu[nt][e] = mu;
@@ -598,8 +599,8 @@ __device__ __forceinline__ void tile_fold(PagedTile<C>& f, uint32_t valid, float
         for (int g = 0; g < C::NG; ++g)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            st.acc[nt][g][i][e] *= al * unit;
-            st.acc[nt][g][i][2 + e] *= al * unit;
+            st.acc[nt][g][i][e] *= al;
+            st.acc[nt][g][i][2 + e] *= al;
           }
       }
   }
@@ -615,16 +616,14 @@ __device__ __forceinline__ void tile_fold(PagedTile<C>& f, uint32_t valid, float
   // O^T += V^T P^T
 #pragma unroll
   for (int mt = 0; mt < C::TT; ++mt) {
-    uint32_t hi[C::NT][2], lo[C::NT][2];  // codes: hi alone
+    uint32_t hi[C::NT][2], lo[C::NT][2];
     auto split = [&](int nt, float w0, float w1, float w2, float w3) {
       const uint32_t h0 = pack16<C::F16>(w0, w1), h1 = pack16<C::F16>(w2, w3);
       hi[nt][0] = trans8x8(h0);
       hi[nt][1] = trans8x8(h1);
-      if constexpr (!C::Q) {
-        const float2 u0 = unpack16<C::F16>(h0), u1 = unpack16<C::F16>(h1);
-        lo[nt][0] = trans8x8(pack16<C::F16>(w0 - u0.x, w1 - u0.y));
-        lo[nt][1] = trans8x8(pack16<C::F16>(w2 - u1.x, w3 - u1.y));
-      }
+      const float2 u0 = unpack16<C::F16>(h0), u1 = unpack16<C::F16>(h1);
+      lo[nt][0] = trans8x8(pack16<C::F16>(w0 - u0.x, w1 - u0.y));
+      lo[nt][1] = trans8x8(pack16<C::F16>(w2 - u1.x, w3 - u1.y));
     };
     if constexpr (!C::Q) {
 #pragma unroll
@@ -644,14 +643,13 @@ __device__ __forceinline__ void tile_fold(PagedTile<C>& f, uint32_t valid, float
         constexpr float mid = C::VB == 8 ? 128.0f : 8.0f;
         const float s0 = scale_of(vs[0], g), s1 = scale_of(vs[1], g);
         const float b0 = __fmaf_rn(mid, s0, scale_of(vb[0], g)), b1 = __fmaf_rn(mid, s1, scale_of(vb[1], g));
-        const float f0 = s0 * st.vf, f1 = s1 * st.vf;
 #pragma unroll
         for (int nt = 0; nt < C::NT; ++nt) {
           const float* pp = x[mt][nt];
 #pragma unroll
           for (int e = 0; e < 2; ++e)
             st.xb[nt][e][g] = __fmaf_rn(pp[e], b0, __fmaf_rn(pp[2 + e], b1, st.xb[nt][e][g]));
-          split(nt, pp[0] * f0, pp[1] * f0, pp[2] * f1, pp[3] * f1);
+          split(nt, pp[0] * s0, pp[1] * s0, pp[2] * s1, pp[3] * s1);
         }
       }
 #pragma unroll
@@ -687,7 +685,7 @@ __device__ __forceinline__ void tile_fold(PagedTile<C>& f, uint32_t valid, float
 #pragma unroll
         for (int nt = 0; nt < C::NT; ++nt) {
           mma16816<C::F16>(st.acc[nt][g][i], A[0], A[1], A[2], A[3], hi[nt][0], hi[nt][1]);
-          if constexpr (!C::Q) mma16816<C::F16>(st.acc[nt][g][i], A[0], A[1], A[2], A[3], lo[nt][0], lo[nt][1]);
+          mma16816<C::F16>(st.acc[nt][g][i], A[0], A[1], A[2], A[3], lo[nt][0], lo[nt][1]);
         }
       }
     }
@@ -868,11 +866,18 @@ __global__ void __launch_bounds__(C::W * 32, C::MINB) k_paged_attn(const PagedVi
             for (int g = 0; g < C::NG; ++g) xb[g] += __shfl_xor_sync(0xffffffffu, xb[g], o);
           }
         }
-        if (j == 0) {
-          sm.m[warp][n] = st.m[nt][e] == -INFINITY ? -INFINITY : st.mu[nt][e];
-          sm.l[warp][n] = l;
+        float M = st.m[nt][e] == -INFINITY ? -INFINITY : st.mu[nt][e], back = 1.0f;
+        if constexpr (C::Q) {
+          if (l != 0.0f) {  // from the slots' scales' units to a sum in [1, 2)
+            const int ex = min(126, max(-126, int(__float_as_uint(l) >> 23 & 255u) - 127));
+            M += float(ex);
+            back = __int_as_float((127 - ex) << 23);
+          }
         }
-        const float back = C::Q ? (st.vf == 0.0f ? 1.0f : 1.0f / st.vf) : 1.0f;
+        if (j == 0) {
+          sm.m[warp][n] = M;
+          sm.l[warp][n] = l * back;
+        }
 #pragma unroll
         for (int g = 0; g < C::NG; ++g) {
           float y[8];
@@ -883,7 +888,7 @@ __global__ void __launch_bounds__(C::W * 32, C::MINB) k_paged_attn(const PagedVi
           }
           if constexpr (C::Q) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = __fmaf_rn(y[i], back, xb[g]);
+            for (int i = 0; i < 8; ++i) y[i] = (y[i] + xb[g]) * back;
           }
           float4* dst = reinterpret_cast<float4*>(&sm.acc[warp][n][64 * g + 8 * j]);
           dst[0] = make_float4(y[0], y[1], y[2], y[3]);

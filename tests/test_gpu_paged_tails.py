@@ -5,7 +5,7 @@ slots, each 2^-20 to 2^-26 of it, bring.
 Bounds.  Scores are exact here (one dim of q is 1, the others 0), so a weight
 is off by the rounding of x * scale * log2(e), below 2^-17 of it, and by ex2's
 2^-22; the MMA's sums add a few 2^-23 each: 2^-14 of sum p |v| covers them.
-The weights of fp16 rows enter the PV product as two
+The weights (times the slot's scale for codes) enter the PV product as two
 fp16 numbers, in units where the largest of them is at least 2^9, on a grid of
 2^-24 at the finest: an error of 2^-34 of that largest one per slot, or 2^-22 of
 the product itself.  Last the output is rounded: 2^-11 (fp16) or 2^-8 (bf16) of
@@ -74,3 +74,40 @@ def test_rows(kind, tail, d):
     k, v = (torch.from_numpy(x).cuda().to(dt) for x in (k, v))
     V = ref.values(v, 16)
     run(paged.PagedKV(k, v), ref.values(k, 16), V, table, np.ones(V.shape[:3]), heads, np.abs(V), dt)
+
+
+@pytest.mark.parametrize("kb,vb", [(8, 8), (8, 4), (4, 8), (4, 4)])
+@pytest.mark.parametrize("code", [4, 2, 0])
+@pytest.mark.parametrize("wide", [0, 6, -20])
+@pytest.mark.parametrize("d", [64, 256])
+def test_codes(kb, vb, code, wide, d):
+    """wide: the dominating slots' scale is 2^wide times the others' (their
+    value is zero all the same: bias = -middle * scale)."""
+    rng = np.random.default_rng(100 * kb + 10 * vb + code)
+    table, pages = ref.page_table(LENGTHS, PAGE, rng)
+    pg, off, big = slots_of(table)
+    heads, groups = 2, d // 64
+    shape = (pages, heads, PAGE)
+    # K: -26.25 .. 0 in steps of 1.75 (4 bits), or the same from every 14th code of 8 bits
+    ks, kbias, top = (1.75, -26.25, 15) if kb == 4 else (0.125, -26.25, 210)
+    kc = rng.integers(0, 1 << kb, (*shape, d))
+    kc[pg, :, off, 0] = np.where(big, top, code if kb == 4 else 14 * code)[:, None]
+    mid = 1 << (vb - 1)
+    vc = rng.integers(0, 1 << vb, (*shape, d))
+    vc[pg[big], :, off[big]] = mid
+    s = np.full((*shape, groups), 1.296875, dtype=np.float32)
+    s *= 2.0 ** rng.integers(-3, 4, s.shape)
+    bias = s * 8
+    s[pg[big], :, off[big]] = 2.0 ** wide
+    bias[pg[big], :, off[big]] = -mid * 2.0 ** wide
+
+    def bf(x):
+        return torch.from_numpy(np.ascontiguousarray(np.broadcast_to(x, (*shape, groups))).astype(np.float32)).cuda().bfloat16()
+
+    k, v = ref.pack(kc, kb).cuda(), ref.pack(vc, vb).cuda()
+    scales = [bf(ks), bf(kbias), bf(s), bf(bias)]
+    cache = paged.PagedKV(k, v, *scales)
+    unit = np.abs(scales[2].double().cpu().numpy())
+    # a product's error times |code - middle|
+    run(cache, ref.values(k, kb, *scales[:2]), ref.values(v, vb, *scales[2:]), table, unit.max(-1), heads,
+        np.abs(vc - mid).astype(np.float64), torch.bfloat16)
