@@ -916,7 +916,8 @@ __global__ void __launch_bounds__(C::W * 32, C::MINB) k_paged_attn(const PagedVi
       if (d == 0 && (a.lse || a.lse2)) {
         const float lse2 = sum == 0.0f ? -INFINITY : ref + log2f(sum);
         if (a.lse) a.lse[s.b * a.hq + hq] = lse2 * kLn2;
-        if (a.lse2) a.lse2[s.b * a.hq + hq] = lse2;
+        // (every score -inf: 2^(-inf - 0) gives the slots no weight)
+        if (a.lse2) a.lse2[s.b * a.hq + hq] = sum == 0.0f ? 0.0f : lse2;
       }
     };
     const int slot = whole ? 0 : 2 * blockIdx.x + (int64_t(blockIdx.x) * sm.per >= head0 ? 0 : 1);
