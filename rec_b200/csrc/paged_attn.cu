@@ -36,7 +36,10 @@ __global__ void __launch_bounds__(kWeightThreads) k_paged_weights(const PagedVie
     if (t >= L) continue;
     int off;
     const int page = slot_page(p, b, t, off);
-    if (page < 0) continue;
+    if (page < 0) {  // (below the window the attention has not looked)
+      report(a.status, kStatusBadPage);
+      continue;
+    }
     float w = 0.0f;
     if (a.window <= 0 || t >= L - a.window) {
       const float* sc = a.scores + (int64_t(b * p.hkv + h) * a.score_len + t) * a.G;

@@ -42,3 +42,27 @@ def test_scores_that_are_all_minus_infinity(dtype, group):
     pg, off = ref.rows_of(table, 2, 40, page)
     for h in range(heads):
         assert abs((got[pg, h, off] - 0.5 * before[pg, h, off]).sum() - group) <= 1e-4
+
+
+@pytest.mark.parametrize("window", [0, 20])
+def test_bad_pages_below_the_window_are_reported(window):
+    """The attention does not look there, the weights do: the slots are left
+    out, and the call is recorded."""
+    page, lengths = 16, np.array([100], dtype=np.int32)
+    table, pages = ref.page_table(lengths, page, np.random.default_rng(2))
+    k = torch.randn(pages, 1, page, 64, device="cuda").bfloat16()
+    q = torch.randn(1, 4, 64, device="cuda").bfloat16()
+    n = torch.from_numpy(lengths).cuda()
+    for bad in (-1, pages):
+        broken = table.copy()
+        broken[0, 2] = bad
+        w = torch.ones(pages, 1, page, device="cuda")
+        paged.paged_attn_decode(paged.PagedKV(k, k), q, torch.from_numpy(broken).cuda(), n, window=window, weights=w,
+                                decay=0.25)
+        with pytest.raises(RuntimeError, match="status 5"):
+            paged.check_status()
+        paged.check_status()
+        assert bool((w[int(table[0, 2])] == 1.0).all()) and bool((w[int(table[0, 0])] != 1.0).all())
+        # without weights, what lies below the window is nobody's
+        paged.paged_attn_decode(paged.PagedKV(k, k), q, torch.from_numpy(broken).cuda(), n, window=20)
+        paged.check_status()
