@@ -6,7 +6,9 @@ row t % page_size of page table[b, t / page_size].  Pools are torch tensors
 that the caller allocates; these calls keep no reference to them.  They are
 ordered on torch's current stream and do not synchronise.  A page id outside
 the pool or a slot outside the table is left out and recorded on the device:
-`check_status` raises for it.
+`check_status` raises for it.  The record is made with a device's first
+PagedKV; a graph that is captured before any was made records nothing, and the
+capture warns.
 
 Scratch memory is kept per (device, stream) and grows with the largest call,
 so calls on different streams do not meet; a call under stream capture takes
@@ -18,6 +20,7 @@ from __future__ import annotations
 import ctypes as C
 import struct
 import threading
+import warnings
 
 import torch
 
@@ -109,6 +112,8 @@ class PagedKV:
         self.k, self.v, self._index = k, v, index
         self.scales = (k_scales, k_biases, v_scales, v_biases)
         self.shape = (pages, heads, page)
+        if index not in _status and not _capturing():
+            _status_ptr(index)  # so that a first call under capture finds it
 
     @property
     def device(self) -> torch.device:
@@ -138,8 +143,10 @@ def _stream(index: int) -> int:
 def _status_ptr(index: int) -> int | None:
     s = _status.get(index)
     if s is None:
-        if _capturing():
-            return None  # cleared by every replay if it were captured
+        if _capturing():  # made here it would be cleared by every replay
+            warnings.warn("bad pages and slots of this capture are not recorded: make a PagedKV before it begins",
+                          RuntimeWarning, stacklevel=3)
+            return None
         t = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", index))
         torch.cuda.current_stream(index).synchronize()  # zero before any other stream's call
         s = _status.setdefault(index, (t, t.data_ptr()))  # the first thread's word
