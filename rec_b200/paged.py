@@ -134,6 +134,13 @@ class PagedKV:
                              for _ in range(4)))
 
 
+def _packed(pack: struct.Struct, *fields) -> bytes:
+    try:
+        return pack.pack(*fields)
+    except struct.error as e:  # a number that the C structure's field does not hold
+        raise ValueError(f"an argument is out of range: {e}") from None
+
+
 def _stream(index: int) -> int:
     if index != _current_device():
         raise ValueError("the tensors must live on the current CUDA device")
@@ -286,9 +293,9 @@ def paged_attn_decode(cache: PagedKV, q: torch.Tensor, table: torch.Tensor, leng
         decay = 0.0
     if weights_out is not None:
         weights_to = _per_slot("weights_out", weights_out, cache, _f32)
-    a = _ATTN.pack(q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1), lse_at,
-                   _ints("lengths", lengths, B, index), sinks_at, hq, d ** -0.5 if scale is None else scale, softcap,
-                   window, weights_at, weights_to, decay)
+    a = _packed(_ATTN, q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1), lse_at,
+                _ints("lengths", lengths, B, index), sinks_at, hq, d ** -0.5 if scale is None else scale, softcap,
+                window, weights_at, weights_to, decay)
     L = lib()
     key = (index, B, width, hq, d, cache.shape, cache.bits, weights_to != 0)
     size = _sizes.get(key)
@@ -339,8 +346,8 @@ def paged_evict(cache: PagedKV, table: torch.Tensor, lengths: torch.Tensor, budg
         positions_to = _per_slot("positions_out", positions_out, cache, _i32)
     if keep_from is not None:
         keep_at = _ints("keep_from", keep_from, B, index)
-    a = _EVICT.pack(_ints("lengths", lengths, B, index), _ints("lengths_out", lengths_out, B, index), budget, weights_at,
-                    weights_to, positions_at, positions_to, keep_at, keep_below)
+    a = _packed(_EVICT, _ints("lengths", lengths, B, index), _ints("lengths_out", lengths_out, B, index), budget,
+                weights_at, weights_to, positions_at, positions_to, keep_at, keep_below)
     L = lib()
     stream = _stream(index)
     need = L.rec_paged_evict_workspace_bytes(cache._desc, t, budget)

@@ -1,0 +1,87 @@
+"""Arguments of the batched calls that the Python side answers for, on the CPU
+with a stand-in for the library."""
+import types
+
+import pytest
+import torch
+
+from rec_b200 import abi, paged
+
+
+class Library:
+    def __init__(self):
+        self.attn, self.evicted = [], []
+
+    def rec_paged_attn_workspace_bytes(self, kv, table, hq, weights, counters):
+        counters._obj.value = 64
+        return 512
+
+    def rec_paged_evict_workspace_bytes(self, kv, table, budget):
+        return 512
+
+    def rec_paged_attn_decode(self, kv, table, a, *rest):
+        self.attn.append(abi.RecPagedAttn.from_buffer_copy(a))
+        return 0
+
+    def rec_paged_evict(self, kv, table, e, *rest):
+        self.evicted.append(abi.RecPagedEvict.from_buffer_copy(e))
+        return 0
+
+
+class Torch:
+    """torch, with devices on the CPU; counts what it allocates."""
+
+    def __init__(self):
+        self.made = 0
+
+    def __getattr__(self, name):
+        return getattr(torch, name)
+
+    def device(self, *_):
+        return torch.device("cpu")
+
+    def empty(self, *a, **k):
+        self.made += 1
+        return torch.empty(*a, **k)
+
+    def zeros(self, *a, **k):
+        self.made += 1
+        return torch.zeros(*a, **k)
+
+
+@pytest.fixture
+def fake(monkeypatch):
+    library = Library()
+    library.torch = Torch()
+    for name, x in dict(lib=lambda: library, torch=library.torch, _scratch={}, _sizes={}, _capturing=lambda: False,
+                        _current_device=lambda: -1, _raw_stream=lambda i: 0, _status_ptr=lambda i: None).items():
+        monkeypatch.setattr(paged, name, x)
+    return library
+
+
+CACHE = types.SimpleNamespace(_index=-1, head_dim=8, dtype=torch.bfloat16, shape=(4, 1, 16), bits=(16, 16), _desc=b"")
+
+
+def attend(batch=2, width=4, heads=8, q=None, **over):
+    q = torch.zeros(batch, heads, 8, dtype=torch.bfloat16) if q is None else q
+    return paged.paged_attn_decode(CACHE, q, torch.zeros(batch, width, dtype=torch.int32),
+                                   torch.zeros(batch, dtype=torch.int32), **over)
+
+
+def evict(budget, batch=2, **over):
+    return paged.paged_evict(CACHE, torch.zeros(batch, 4, dtype=torch.int32), torch.zeros(batch, dtype=torch.int32), budget,
+                             torch.zeros(4, 1, 16), **over)
+
+
+@pytest.mark.parametrize("call", [lambda: attend(window=2 ** 31), lambda: attend(window=-2 ** 40), lambda: evict(2 ** 31),
+                                  lambda: evict(-2 ** 31 - 1), lambda: evict(4, keep_below=2 ** 33)])
+def test_numbers_out_of_range_are_value_errors(fake, call):
+    with pytest.raises(ValueError, match="out of range"):
+        call()
+    assert not fake.attn and not fake.evicted
+
+
+def test_the_largest_numbers_pass(fake):
+    attend(window=2 ** 31 - 1, scale=1e30)
+    evict(2 ** 31 - 1, keep_below=2 ** 31 - 1)
+    assert fake.attn[0].window == fake.evicted[0].budget == fake.evicted[0].keep_below == 2 ** 31 - 1
