@@ -85,3 +85,14 @@ def test_the_largest_numbers_pass(fake):
     attend(window=2 ** 31 - 1, scale=1e30)
     evict(2 ** 31 - 1, keep_below=2 ** 31 - 1)
     assert fake.attn[0].window == fake.evicted[0].budget == fake.evicted[0].keep_below == 2 ** 31 - 1
+
+
+def test_an_eviction_has_no_counters(fake, monkeypatch):
+    """Under capture they would be cleared by every replay for nothing."""
+    lengths = torch.zeros(2, dtype=torch.int32)
+    for capturing in (False, True):
+        monkeypatch.setattr(paged, "_capturing", lambda: capturing)
+        fake.torch.made = 0
+        evict(16, lengths_out=lengths)
+        # the workspace, and the tensors that this file's `evict` makes through torch itself are not counted
+        assert fake.torch.made == 1
