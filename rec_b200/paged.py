@@ -293,9 +293,13 @@ def paged_attn_decode(cache: PagedKV, q: torch.Tensor, table: torch.Tensor, leng
         decay = 0.0
     if weights_out is not None:
         weights_to = _per_slot("weights_out", weights_out, cache, _f32)
-    a = _packed(_ATTN, q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1), lse_at,
-                _ints("lengths", lengths, B, index), sinks_at, hq, d ** -0.5 if scale is None else scale, softcap,
-                window, weights_at, weights_to, decay)
+    (q0, q1, _), (o0, o1, _) = q.stride(), out.stride()
+    if B == 1:  # a single session's or head's stride is never used
+        q0 = o0 = 0
+    if hq == 1:
+        q1 = o1 = 0
+    a = _packed(_ATTN, q.data_ptr(), q0, q1, out.data_ptr(), o0, o1, lse_at, _ints("lengths", lengths, B, index), sinks_at,
+                hq, d ** -0.5 if scale is None else scale, softcap, window, weights_at, weights_to, decay)
     L = lib()
     key = (index, B, width, hq, d, cache.shape, cache.bits, weights_to != 0)
     size = _sizes.get(key)

@@ -96,3 +96,14 @@ def test_an_eviction_has_no_counters(fake, monkeypatch):
         evict(16, lengths_out=lengths)
         # the workspace, and the tensors that this file's `evict` makes through torch itself are not counted
         assert fake.torch.made == 1
+
+
+@pytest.mark.parametrize("batch,heads,strides", [(1, 8, (3, 8, 1)), (2, 1, (8, 5, 1)), (1, 1, (3, 5, 1)), (2, 8, (64, 8, 1))])
+def test_strides_that_no_address_uses_are_not_checked(fake, batch, heads, strides):
+    """A dimension of one entry may have any stride (a slice, an expanded
+    view); the library wants multiples of 8 elements."""
+    q, out = (torch.zeros(256, dtype=torch.bfloat16).as_strided((batch, heads, 8), strides) for _ in range(2))
+    attend(batch=batch, q=q, out=out)
+    a = fake.attn[0]
+    for got in ((a.q_batch_stride, a.q_head_stride), (a.out_batch_stride, a.out_head_stride)):
+        assert got == (strides[0] if batch > 1 else 0, strides[1] if heads > 1 else 0)
