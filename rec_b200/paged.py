@@ -235,7 +235,7 @@ def paged_append(cache: PagedKV, k: torch.Tensor, v: torch.Tensor, table: torch.
     if k.dtype != dtype or v.dtype != dtype or k.shape != want or v.shape != want \
             or k.get_device() != index or v.get_device() != index or k2 != 1 or v2 != 1 or (heads > 1 and (k1 != d or v1 != d)):
         raise ValueError(f"k and v must be {dtype} [rows, {heads}, {d}] on the cache's device, each row contiguous")
-    if rows == 0:
+    if rows == 0 or B == 0:
         return
     if rows == 1:  # a single row's stride is never used
         k0 = v0 = heads * d
@@ -300,6 +300,8 @@ def paged_attn_decode(cache: PagedKV, q: torch.Tensor, table: torch.Tensor, leng
         q1 = o1 = 0
     a = _packed(_ATTN, q.data_ptr(), q0, q1, out.data_ptr(), o0, o1, lse_at, _ints("lengths", lengths, B, index), sinks_at,
                 hq, d ** -0.5 if scale is None else scale, softcap, window, weights_at, weights_to, decay)
+    if B == 0:
+        return out
     L = lib()
     key = (index, B, width, hq, d, cache.shape, cache.bits, weights_to != 0)
     size = _sizes.get(key)
@@ -352,6 +354,8 @@ def paged_evict(cache: PagedKV, table: torch.Tensor, lengths: torch.Tensor, budg
         keep_at = _ints("keep_from", keep_from, B, index)
     a = _packed(_EVICT, _ints("lengths", lengths, B, index), _ints("lengths_out", lengths_out, B, index), budget,
                 weights_at, weights_to, positions_at, positions_to, keep_at, keep_below)
+    if B == 0:
+        return lengths_out
     L = lib()
     stream = _stream(index)
     need = L.rec_paged_evict_workspace_bytes(cache._desc, t, budget)

@@ -107,3 +107,17 @@ def test_strides_that_no_address_uses_are_not_checked(fake, batch, heads, stride
     a = fake.attn[0]
     for got in ((a.q_batch_stride, a.q_head_stride), (a.out_batch_stride, a.out_head_stride)):
         assert got == (strides[0] if batch > 1 else 0, strides[1] if heads > 1 else 0)
+
+
+def test_an_empty_batch_is_nothing_to_do(fake):
+    """As for process_logits; arguments that do not match are still refused."""
+    assert attend(batch=0).shape == (0, 8, 8)
+    assert evict(16, batch=0).shape == (0,)
+    rows = torch.zeros(0, 1, 8, dtype=torch.bfloat16)
+    none, cu = torch.zeros(0, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    paged.paged_append(CACHE, rows, rows, torch.zeros(0, 4, dtype=torch.int32), none, cu)
+    assert not fake.attn and not fake.evicted and fake.torch.made == 0
+    with pytest.raises(ValueError):
+        attend(batch=0, lse=torch.zeros(1, 8))
+    with pytest.raises(ValueError):
+        evict(2 ** 40, batch=0)
