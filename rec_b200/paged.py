@@ -310,6 +310,8 @@ def paged_attn_decode(cache: PagedKV, q: torch.Tensor, table: torch.Tensor, leng
         need = L.rec_paged_attn_workspace_bytes(cache._desc, t, hq, weights_to != 0, C.byref(zero))
         size = (need, zero.value)
         if need:
+            if len(_sizes) >= 4096:  # a server's batches and widths vary without end
+                _sizes.clear()
             _sizes[key] = size
     stream = _stream(index)
     with _lock:

@@ -121,3 +121,9 @@ def test_an_empty_batch_is_nothing_to_do(fake):
         attend(batch=0, lse=torch.zeros(1, 8))
     with pytest.raises(ValueError):
         evict(2 ** 40, batch=0)
+
+
+def test_the_remembered_sizes_are_bounded(fake):
+    for width in range(5000):
+        attend(batch=1, width=width + 1, heads=1)
+    assert 0 < len(paged._sizes) <= 4096 and len(fake.attn) == 5000
