@@ -50,6 +50,7 @@ for _pack, _type in ((_KV, abi.RecPagedKV), (_TABLE, abi.RecPagedTable), (_ATTN,
     assert _pack.size == C.sizeof(_type), _type
 
 _bf16, _f32, _i32 = torch.bfloat16, torch.float32, torch.int32
+_WORDS = (torch.int32, torch.uint32)  # of codes
 _capturing = torch.cuda.is_current_stream_capturing
 
 
@@ -88,7 +89,7 @@ class PagedKV:
             self._desc = _KV.pack(k.data_ptr(), v.data_ptr(), 0, 0, 0, 0, 2 * k0, 2 * k1, 2 * k2, 2 * v0, 2 * v1, 2 * v2,
                                   0, 0, 0, 0, 0, 0, pages, page, heads, kw, 16, 16, kind)
         else:
-            if k.element_size() != 4 or v.element_size() != 4 or k_scales is None or k_biases is None \
+            if dtype not in _WORDS or v.dtype not in _WORDS or k_scales is None or k_biases is None \
                     or v_scales is None or v_biases is None:
                 raise ValueError("pools must be bf16, fp16, or 32-bit code words with scales and biases")
             shape, a, b = k_scales.shape, k_scales.stride(), v_scales.stride()
