@@ -267,7 +267,7 @@ def process_logits(logits: torch.Tensor, history: torch.Tensor | None = None,
         m = bias_ids.shape[1]
         ids_at, values_at = bias_ids.data_ptr(), bias_values.data_ptr()
     if allow is not None:
-        if allow.element_size() != 4 or allow.dim() != 2 or allow.shape[0] != B or allow.get_device() != index \
+        if allow.dtype not in (torch.int32, torch.uint32) or allow.dim() != 2 or allow.shape[0] != B or allow.get_device() != index \
                 or allow.stride(1) != 1 or allow.shape[1] < (V + 31) // 32:
             raise ValueError("allow must be 32-bit words [B, >= ceil(V / 32)] on the logits' device, rows contiguous")
         allow_at, allow_stride = allow.data_ptr(), allow.stride(0)
