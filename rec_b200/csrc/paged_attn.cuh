@@ -8,11 +8,13 @@
 // its share segment by segment (a segment: its units of one (session, head));
 // a segment that is not the whole list of its head leaves a partial state,
 // and the last block to finish a head joins the partials in block order.  A
-// join takes about as long as two units (3.5 us), so where every head can have
-// a block of its own and none is longer than that beyond an even share, a
-// block takes a whole head (24 sessions, window 513: 14.6 -> 9.4 us; 300 slots
-// 9.5 -> 8.0; 500 slots 10.5 -> 10.1; 800 slots of 8-bit codes 11.2 -> 11.9;
-// three more units instead of two would make no difference).
+// join takes 2 to 3.5 us, as long as one or two units, so where every head can
+// have a block of its own and none is longer than WHOLE units beyond an even
+// share, a block takes a whole head.  One session with 4 kv heads, split and
+// whole: 300 slots of bf16 9.4 and 8.1 us, 600 slots of 8-bit codes 10.6 and
+// 10.1 (one more unit); 450 slots of fp16, 64 dims, 8.4 and 7.4 (two more).  A
+// second unit more costs where a unit is long: 800 slots of 8-bit codes 10.9
+// split, 12.1 whole (units of 384 slots), 300 of bf16, 256 dims, 11.3 and 11.9.
 //
 // Tile.  A warp folds 16 * TT slots at a time on the tensor cores
 // (mma.m16n8k16), with the cache as the A operand so that 8 query heads fill
@@ -180,6 +182,8 @@ struct PagedCfg {
   // MMAs take p from 2^9 (at the maximum) up to 2^14 (codes: p * scale, below 2^15), bf16 needs no such place.
   // (LAG 2 and REF 11 would gain two bits and cost codes 0.5 %.)
   static constexpr float LAG = F16 ? 4.0f : 8.0f, REF = F16 ? 9.0f : 0.0f;
+  // Units beyond an even share up to which a block takes a whole head.
+  static constexpr int WHOLE = TT == 2 || (!Q && DP == 256) ? 1 : 2;
 };
 
 template <class C>
@@ -757,7 +761,7 @@ __global__ void __launch_bounds__(C::W * 32, C::MINB) k_paged_attn(const PagedVi
   {
     int64_t per = (pre[p.batch] * H + gridDim.x - 1) / gridDim.x;
     if (int64_t(p.batch) * H <= gridDim.x) {
-      const int b = threadIdx.x, nb = b < p.batch ? pre[b + 1] - pre[b] : 0, most = int(per) + 2;
+      const int b = threadIdx.x, nb = b < p.batch ? pre[b + 1] - pre[b] : 0, most = int(per) + C::WHOLE;
       for (int k = int(per); k <= most; ++k)
         if (!__syncthreads_or(nb > k)) {  // every head's units filled up to k: a block's share is a head
           if (b <= p.batch) pre[b] = b * k;
