@@ -166,16 +166,17 @@ def _buffers(call: str, index: int, stream: int, need: int, zero: int) -> tuple:
     the tensors, which the caller holds until the launch, and (address, bytes,
     address, bytes).  Called with the lock held."""
     s = _scratch.get((call, index, stream))
-    if s is not None and s[1][1] >= need and s[1][3] >= zero and not _capturing():
+    capturing = _capturing()
+    if s is not None and s[1][1] >= need and s[1][3] >= zero and not capturing:
         return s
     device = torch.device("cuda", index)
     need, zero = max(need, 256), max(zero, 4096) if zero else 0
-    if s is not None:
+    if s is not None and not capturing:
         need, zero = max(need, s[1][1]), max(zero, s[1][3])
     ws = torch.empty(need, dtype=torch.uint8, device=device)
     counters = torch.zeros(zero, dtype=torch.uint8, device=device) if zero else None
     s = ((ws, counters), (ws.data_ptr(), need, counters.data_ptr() if zero else 0, zero))
-    if not _capturing():
+    if not capturing:
         _scratch[(call, index, stream)] = s
     return s
 

@@ -127,3 +127,15 @@ def test_the_remembered_sizes_are_bounded(fake):
     for width in range(5000):
         attend(batch=1, width=width + 1, heads=1)
     assert 0 < len(paged._sizes) <= 4096 and len(fake.attn) == 5000
+
+
+def test_a_captured_call_takes_what_it_needs(fake, monkeypatch):
+    """Not the size of the largest call so far, which a graph would keep."""
+    sizes = []
+    monkeypatch.setattr(fake, "rec_paged_evict_workspace_bytes", lambda kv, table, budget: 1000 * budget)
+    monkeypatch.setattr(fake, "rec_paged_evict", lambda kv, table, e, ws, n, *rest: sizes.append(n) or 0)
+    evict(900)
+    evict(5)
+    monkeypatch.setattr(paged, "_capturing", lambda: True)
+    evict(5)
+    assert sizes == [900000, 900000, 5000]
