@@ -556,13 +556,18 @@ REC_API int rec_paged_append(const RecPagedKV* kv, const RecPagedTable* table, c
  *   s_t = scale * q . k_t, or softcap * tanh(s_t / softcap) for softcap > 0;
  *   t in [max(0, L - window), L) (window 0: all); softmax over them with the
  *   head's sink logit in the denominator when sinks are given;
- *   out = sum p_t v_t; a session with no slot gives zeros and lse -inf.
+ *   out = sum p_t v_t; lse = log of the denominator, the sink's part included.
+ * A session with no slot, or whose every score is -inf, gives zeros, its lse
+ * is -inf (with sinks: the sink's logit) and its slots get no weight.  The
+ * window counts slots: after an eviction the last slots are not the last
+ * tokens.
  * With weights_out, every slot t < L also gets
  *   weights_out[t] = decay * weights_in[t] + sum of p_t over the kv head's
  *   query heads   (weights_in may be weights_out; decay 0 reads nothing).
  * The slots that take weights belong to one session each: sessions that share
  * pages would overwrite one another's sums.
- * A page outside the pool sets *status_dev and its slots are left out. */
+ * A page outside the pool sets *status_dev and its slots are left out (pages
+ * wholly below the window are looked at for weights_out only). */
 typedef struct RecPagedAttn {
   const void* q;            /* [batch][n_q_heads][head_dim], 16-byte aligned */
   int64_t q_batch_stride, q_head_stride;     /* elements, multiples of 8 */
@@ -579,7 +584,10 @@ typedef struct RecPagedAttn {
   float decay;
 } RecPagedAttn;
 /* Workspace bytes of rec_paged_attn_decode (weights: non-zero when
- * weights_out is given); 0 for bad arguments.  *counter_bytes: the size of its
+ * weights_out is given); 0 for bad arguments.  With weights it holds a score
+ * per query head and slot of the page table, 4 * batch * n_q_heads * width *
+ * page_size bytes whatever the lengths are (batch * width * page_size is at
+ * most 2^37): a table no wider than its longest session keeps it small.  *counter_bytes: the size of its
  * counters, a buffer of their own that is zero before the first call and that
  * every call, of any shape, leaves zero.  Calls that overlap on the GPU need
  * a workspace and counters of their own. */
@@ -598,7 +606,8 @@ REC_API int rec_paged_attn_decode(const RecPagedKV* kv, const RecPagedTable* tab
  * there are such slots.  positions_in NULL: a slot's position is its number.
  * weights_out / positions_out / lengths_out may be the inputs; each slot
  * below min(budget, L) is written, positions_out may be NULL when
- * positions_in is.  The pages below the budget must belong to one session. */
+ * positions_in is.  The pages below the budget must belong to one session.
+ * batch * n_kv_heads is at most 65,535. */
 typedef struct RecPagedEvict {
   const int32_t* lengths;
   int32_t* lengths_out;

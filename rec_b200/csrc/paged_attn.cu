@@ -26,7 +26,8 @@ __global__ void __launch_bounds__(kWeightThreads) k_paged_weights(const PagedVie
   int* pre = plan + p.batch;
   plan_units(p, a.lengths, nullptr, kWeightThreads, len, pre, scan,
              [](int L) { return max(1, (L + kWeightThreads - 1) / kWeightThreads); });
-  grid_wait();  // launched while the attention ends; what it wrote is read by plain loads, which stay below
+  // launched once the attention's last block has left; what it wrote is read by plain loads, which stay below
+  grid_wait();
   const int64_t H = p.hkv, total = pre[p.batch] * H;
   for (int64_t u = blockIdx.x; u < total; u += gridDim.x) {
     const int b = unit_session(pre, p.batch, H, u);

@@ -333,7 +333,7 @@ constexpr int kMoveThreads = 256;
 // A warp takes M moves at a time.
 template <int M>
 __global__ void __launch_bounds__(kMoveThreads) k_evict_move(const PagedView p, const EvictArgs a, const FastDiv per) {
-  grid_wait();  // launched while the selection ends
+  grid_wait();  // launched once the selection's last block has left
   const int row = blockIdx.y, b = row / p.hkv, h = row - b * p.hkv, lane = threadIdx.x & 31;
   if (blockIdx.x == 0 && h == 0 && threadIdx.x == 0) {
     const int64_t L = max(0, a.lengths[b]);

@@ -10,8 +10,8 @@ the pool or a slot outside the table is left out and recorded on the device:
 PagedKV; a graph that is captured before any was made records nothing, and the
 capture warns.
 
-Scratch memory is kept per (device, stream) and grows with the largest call,
-so calls on different streams do not meet; a call under stream capture takes
+Scratch memory is kept per (device, stream) for the life of the process and
+grows with the largest call, so calls on different streams do not meet; a call under stream capture takes
 its scratch from the capture's own pool.  Threads may share a stream: a lock
 keeps one call's launches together.
 """
@@ -262,13 +262,17 @@ def paged_attn_decode(cache: PagedKV, q: torch.Tensor, table: torch.Tensor, leng
 
     Scores are scale (default head_dim ** -0.5) * q . k, capped as softcap *
     tanh(s / softcap) when softcap > 0; window > 0 attends the last `window`
-    slots only; sinks (bf16 [query heads]) join the softmax's denominator.  A
-    session with no slot gives zeros.  lse (fp32 [batch, query heads], natural
-    log) is filled when given.  weights (fp32, one value per slot) accumulate:
+    slots only, which are the last tokens until the session's first eviction;
+    sinks (bf16 [query heads]) join the softmax's denominator.  A session with
+    no slot gives zeros.  lse (fp32 [batch, query heads], natural log, the sink
+    included) is filled when given.  weights (fp32, one value per slot) accumulate:
     weights_out = decay * weights + the slot's softmax weights summed over the
     kv head's query heads, for every slot below the session's length;
     weights_out defaults to weights (in place).  Slots that take weights belong
-    to one session each."""
+    to one session each.  Such a call keeps a score per query head and slot of
+    the page table, 4 * batch * query heads * width * page_size bytes of scratch
+    whatever the lengths are: 1.07 GB for 64 sessions of 32 heads and a table of
+    131,072 slots.  Slice the table to the longest session where that counts."""
     index, d = cache._index, cache.head_dim
     t, B, width = _table(table, index)
     shape = q.shape
