@@ -619,6 +619,9 @@ typedef struct RecPagedEvict {
   const int32_t* keep_from; /* [batch] or NULL */
   int32_t keep_below;
 } RecPagedEvict;
+/* Each call launches two kernels that meet in the workspace, as
+ * rec_paged_attn_decode with weights does: threads that share a stream and a
+ * workspace call one at a time. */
 REC_API size_t rec_paged_evict_workspace_bytes(const RecPagedKV* kv, const RecPagedTable* table, int32_t budget);
 REC_API int rec_paged_evict(const RecPagedKV* kv, const RecPagedTable* table, const RecPagedEvict* evict,
                             void* workspace, size_t workspace_bytes, int32_t* status_dev, void* stream);
